@@ -432,6 +432,147 @@ int qtts_prefill_custom_voice(qtts_ctx *ctx, const uint32_t *text_tokens, int64_
                               float *hidden_out, float *logits_out, int64_t *position_out,
                               int flags);
 
+/* ---- many sequences over a 4-bit cache -------------------------------- */
+
+/* No reference counterpart (the reference decodes one utterance over f32
+ * Vecs): what a program that serves many utterances at once calls between the
+ * q|k|v and the o-proj linear maps (qtts_gemm_q4_noalloc), layer by layer.
+ *
+ * The calls of this section take DEVICE pointers, allocate nothing and only
+ * enqueue kernels on `stream`: a hipStream_t of the context's device (NULL:
+ * that device's default stream; qtts_stream for the context's own).  They may
+ * be captured into a graph.  They leave the caller's current device as it is,
+ * and touch nothing of the context but its last error.  Workspaces are the
+ * caller's: two calls that may run at the same time, graph replays among them,
+ * need two.
+ *
+ * With QTTS_CHECK_ONLY the arguments are checked and nothing is enqueued; ctx
+ * may then be NULL and no device is needed. */
+#define QTTS_CHECK_ONLY 8
+#define QTTS_F32  0               /* element types of q, k, v rows          */
+#define QTTS_F16  1
+#define QTTS_BF16 2
+
+/* One layer's pages of 64 positions.  Page i holds at base + i * page_stride,
+ * for each kv head in turn, a block of 72 * head_dim bytes (D = head_dim, p a
+ * position in the page):
+ *   K codes   [p % 4][p / 4][D / 2 bytes]   low nibble = even column
+ *   V codes   [p / 4][D / 4][p % 4] 16 bit  four codes, lowest bits first
+ *   K scales  [D / 32][64] f16
+ *   V scales  [D / 32][64] f16
+ * value = (nibble - 8) * scale, as in the Q4 weights; groups of 32 columns.
+ * A scale is -1/8 of the group's value of largest magnitude (the positive one
+ * of two), rounded to f16 and then to 8 significant bits, which makes every
+ * value exact in f16; the nibble is the nearest step (halves to even), at
+ * most 15.  Magnitudes beyond 65280 are stored as 65280. */
+#define QTTS_KV4_PAGE 64
+typedef struct qtts_kv4 {
+    void   *base;                 /* device, 16-byte aligned                */
+    int64_t n_pages;
+    int64_t page_stride;          /* bytes, multiple of 16, at least n_kv_heads * 72 * head_dim */
+    int32_t n_kv_heads, head_dim; /* head_dim 64 or 128                     */
+} qtts_kv4;
+
+/* Block tables and slots of one step from the requests' lengths, in one
+ * launch.  Sequence b holds cached[b] positions in the first
+ * ceil(cached[b] / 64) pages of its table row and adds fresh[b] (0 allowed);
+ * the pages it needs beyond those are taken from free_pages in order,
+ * sequence by sequence, and written into its row.  The step's rows are
+ * packed: sequence b's are row_start[b] .. row_start[b + 1] - 1, and row r
+ * gets its position and its slot (page * 64 + position % 64).  Rows behind
+ * the last sequence get -1 for both.  status[0] is QTTS_OK and status[1] the
+ * pages taken.  Where a length is negative (QTTS_ERR_INVALID) or rows, table
+ * columns or free pages do not suffice (QTTS_ERR_CAPACITY), status[0] says
+ * so, no page is taken, the table stays, all row_start and lengths are 0 and
+ * all rows are -1.  Outputs must not overlap inputs. */
+typedef struct qtts_kv4_tables_args {
+    int32_t n_seqs;               /* at most 4096                           */
+    int32_t max_pages;            /* columns of the table                   */
+    const int32_t *cached;        /* [n_seqs]                               */
+    const int32_t *fresh;         /* [n_seqs]                               */
+    const int32_t *free_pages;    /* [n_free]                               */
+    int64_t n_free;
+    int32_t *table;               /* [n_seqs][table_stride], in and out     */
+    int64_t table_stride;         /* elements, at least max_pages           */
+    int32_t *row_start;           /* [n_seqs + 1] out                       */
+    int32_t *lengths;             /* [n_seqs] out: cached + fresh           */
+    int32_t *positions;           /* [n_rows] out                           */
+    int64_t *slots;               /* [n_rows] out                           */
+    int64_t n_rows;               /* rows there is room for                 */
+    int32_t *status;              /* [2] out                                */
+} qtts_kv4_tables_args;
+int qtts_kv4_tables(qtts_ctx *ctx, const qtts_kv4_tables_args *a, void *stream, int flags);
+
+/* Each head of q and k divided by its root mean square and weighted, then
+ * rotated (pairs i, i + head_dim / 2; row `position` of the tables), in one
+ * pass; with a cache, k so treated and v as it is are stored at the rows'
+ * slots in the same pass.  q_out may be q and k_out may be k (same stride).
+ * A null norm weight leaves the norm out, null positions the rotation.  A row
+ * with a negative position is left out: its outputs stay as they were and
+ * nothing is stored.  A position past the tables makes q and k NaN.  A slot
+ * outside the pages stores nothing; two rows of one call must not share one.
+ * Where k or v of a head holds a NaN, the stored position reads as k NaN and
+ * v 0: attention rows that see it are NaN, the others are not touched. */
+typedef struct qtts_qk_norm_rope_args {
+    int32_t dtype;                /* of q, k, v, q_out, k_out               */
+    int32_t n_heads, n_kv_heads, head_dim;
+    int64_t rows;
+    const void *q, *k, *v;        /* [rows][heads][head_dim], row strides below; v only with a cache */
+    int64_t q_stride, k_stride, v_stride;    /* elements                    */
+    void *q_out, *k_out;          /* k_out may be null with a cache         */
+    int64_t q_out_stride, k_out_stride;
+    const uint16_t *q_norm, *k_norm;         /* [head_dim] f16, or null     */
+    float eps;
+    int32_t reserved;             /* 0                                      */
+    const float *rope_cos, *rope_sin;        /* [rope_max_pos][head_dim/2]  */
+    int64_t rope_max_pos;
+    const int32_t *positions;     /* [rows], or null                        */
+    const qtts_kv4 *cache;        /* null: nothing stored                   */
+    const int64_t *slots;         /* [rows], with a cache                   */
+} qtts_qk_norm_rope_args;
+int qtts_qk_norm_rope(qtts_ctx *ctx, const qtts_qk_norm_rope_args *a, void *stream, int flags);
+
+/* The values held at n slots: K and V [n][n_kv_heads][head_dim] of `dtype`
+ * (exact in f32 and f16; bf16 rounds), zero for a slot outside the pages.
+ * Either may be null.  The counterpart of qtts_kv_gather. */
+int qtts_kv4_gather(qtts_ctx *ctx, const qtts_kv4 *cache, const int64_t *slots, int64_t n,
+                    int32_t dtype, void *K, void *V, void *stream, int flags);
+
+/* out = softmax(scale * q K^T) V of each row and head over its sequence's
+ * pages.  Rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
+ * sequence b's lengths[b]; a row at position i sees positions j <= i, and
+ * only j > i - window with a window.  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  A row that sees nothing is 0; rows outside all
+ * sequences stay as they were.  A table entry outside the pages makes the
+ * rows that see it NaN; entries of pages that no row sees are not read.  Out
+ * may be q (same stride).  max_len, an upper bound of the lengths, says how
+ * far to split the work; a wrong one costs time only.  One row per sequence
+ * is the decode step, many are a prompt; sequences may differ.
+ *
+ * qtts_kv4_attention_workspace: the bytes of device memory (16-byte aligned)
+ * that such a call needs, 0 for many; needs no device. */
+typedef struct qtts_kv4_attention_args {
+    int32_t dtype;                /* of q and out                           */
+    int32_t n_heads;
+    int64_t rows;
+    const void *q;                /* [rows][n_heads][head_dim], row stride q_stride */
+    void *out;
+    int64_t q_stride, out_stride; /* elements                               */
+    const qtts_kv4 *cache;
+    int32_t n_seqs, max_pages;
+    const int32_t *row_start;     /* [n_seqs + 1]                           */
+    const int32_t *lengths;       /* [n_seqs]                               */
+    const int32_t *table;         /* [n_seqs][table_stride]                 */
+    int64_t table_stride;
+    int64_t max_len;
+    float scale;
+    int32_t window;               /* 0: none                                */
+    void *workspace;
+    int64_t workspace_bytes;
+} qtts_kv4_attention_args;
+int qtts_kv4_attention_workspace(const qtts_kv4_attention_args *a, int64_t *bytes);
+int qtts_kv4_attention(qtts_ctx *ctx, const qtts_kv4_attention_args *a, void *stream, int flags);
+
 /* ---- speech decoder --------------------------------------------------- */
 
 /* Upload the speech decoder (codes -> 24 kHz waveform).  Replaces holding

@@ -1,0 +1,893 @@
+// qtts_kv4.hip — serving many sequences over a paged cache held in 4 bits:
+//
+//   k_kv4_tables       block tables, positions and slots of a step
+//   k_qk_norm_rope     norms and rotation of q and k, k and v into the cache
+//   k_kv4_gather       the values held at given slots
+//   k_kv4_attn         attention over the pages, 16 columns a wave
+//   k_kv4_attn_join    its partial results joined
+//
+// The layout of a page's block is in qtts_kv4.h.  A value is (code - 8) *
+// scale with a scale of 8 significant bits, so it has at most 11 and is exact
+// in f16: the matrix cores multiply what the cache stands for, not a rounding
+// of it.
+
+#include "qtts_kv4.h"
+#include "../../include/qtts.h"
+#include "qtts_devutil.h"
+#include "qtts_mfma.h"
+
+#include <algorithm>
+
+namespace qtts {
+
+// ---------------------------------------------------------------------------
+// rows of f32, f16 or bf16
+// ---------------------------------------------------------------------------
+
+// four elements; vec: the address allows one load of them
+template <class T>
+__device__ __forceinline__ f32x4 load4(const T *p, bool vec)
+{
+    typedef T V __attribute__((ext_vector_type(4)));
+    V v;
+    if (vec) {
+        v = *(const V *)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = p[i];
+    }
+    return __builtin_convertvector(v, f32x4);
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T *p, f32x4 x, bool vec)
+{
+    typedef T V __attribute__((ext_vector_type(4)));
+    const V v = __builtin_convertvector(x, V);
+    if (vec) {
+        *(V *)p = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = v[i];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// k_kv4_tables
+// ---------------------------------------------------------------------------
+
+// Every workgroup sums all sequences' rows and pages into LDS (8 bytes a
+// sequence, from cache after the first) and then writes its own part of the
+// rows and of the table: one launch, no workgroup waits for another.  All
+// come to the same verdict on whether the step fits.  The entries that are
+// read (a sequence's last partial page) are never the ones that are written.
+__global__ void __launch_bounds__(1024)
+k_kv4_tables(Kv4Tables a)
+{
+    __shared__ int32_t rs[KV4_MAX_SEQS + 1], ps[KV4_MAX_SEQS + 1];
+    __shared__ int64_t wave_rows[16], wave_pages[16];
+    __shared__ int32_t bad;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    constexpr int PER = KV4_MAX_SEQS / 1024;
+    if (t == 0) bad = 0;
+    __syncthreads();
+    // thread t sums sequences PER t .. PER t + PER - 1
+    int32_t n[PER], pg[PER];
+    int64_t rows = 0, pages = 0;
+    int worst = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int b = t * PER + i;
+        n[i] = pg[i] = 0;
+        if (b >= a.n_seqs) continue;
+        const int64_t c = a.cached[b], f = a.fresh[b];
+        if (c < 0 || f < 0) {
+            worst = QTTS_ERR_INVALID;
+            continue;
+        }
+        const int64_t total = (c + f + KV4_PAGE - 1) / KV4_PAGE;
+        if (total > a.max_pages || f > a.n_rows) {
+            worst = worst ? worst : QTTS_ERR_CAPACITY;
+            continue;
+        }
+        n[i] = (int32_t)f;
+        pg[i] = (int32_t)(total - (c + KV4_PAGE - 1) / KV4_PAGE);
+        rows += n[i];
+        pages += pg[i];
+    }
+    int64_t r = rows, p = pages;     // inclusive sums over the wave, then over the waves
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t r2 = __shfl_up(r, d), p2 = __shfl_up(p, d);
+        if (lane >= d) r += r2, p += p2;
+    }
+    if (lane == 63) wave_rows[wave] = r, wave_pages[wave] = p;
+    // one verdict for all: a negative length before a lack of room
+    if (worst) atomicMin(&bad, worst == QTTS_ERR_INVALID ? -2 : -1);
+    __syncthreads();
+    int64_t all_rows = 0, all_pages = 0;
+    r -= rows;
+    p -= pages;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        if (w < wave) r += wave_rows[w], p += wave_pages[w];
+        all_rows += wave_rows[w];
+        all_pages += wave_pages[w];
+    }
+    const int status = bad == -2 ? QTTS_ERR_INVALID
+                       : bad == -1 || all_rows > a.n_rows || all_pages > a.n_free ? QTTS_ERR_CAPACITY : QTTS_OK;
+    const bool ok = status == QTTS_OK;
+    if (!ok) all_rows = all_pages = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int b = t * PER + i;
+        if (b < a.n_seqs) rs[b] = ok ? (int32_t)r : 0, ps[b] = ok ? (int32_t)p : 0;
+        r += n[i];
+        p += pg[i];
+    }
+    if (t == 0) rs[a.n_seqs] = (int32_t)all_rows, ps[a.n_seqs] = (int32_t)all_pages;
+    __syncthreads();
+
+    const int64_t first = (int64_t)blockIdx.x * 1024 + t, step = (int64_t)gridDim.x * 1024;
+    for (int64_t b = first; b <= a.n_seqs; b += step) {
+        a.row_start[b] = rs[b];
+        if (b < a.n_seqs) a.lengths[b] = ok ? a.cached[b] + a.fresh[b] : 0;
+    }
+    if (first == 0) {
+        a.status[0] = status;
+        a.status[1] = (int32_t)all_pages;
+    }
+    // the last sequence whose sum is at most x: it holds element x
+    const auto owner = [&](const int32_t *sum, int32_t x) {
+        int lo = 0, hi = a.n_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sum[mid] <= x) lo = mid; else hi = mid;
+        }
+        return lo;
+    };
+    for (int64_t row = first; row < a.n_rows; row += step) {
+        int32_t pos = -1;
+        int64_t slot = -1;
+        if (row < all_rows) {
+            const int b = owner(rs, (int32_t)row);
+            const int32_t c = a.cached[b], old = (c + KV4_PAGE - 1) / KV4_PAGE;
+            pos = c + (int32_t)row - rs[b];
+            const int32_t col = pos / KV4_PAGE;
+            const int32_t page = col < old ? a.table[b * a.table_stride + col] : a.free_pages[ps[b] + col - old];
+            slot = page < 0 ? -1 : (int64_t)page * KV4_PAGE + pos % KV4_PAGE;
+        }
+        a.positions[row] = pos;
+        a.slots[row] = slot;
+    }
+    for (int64_t i = first; i < all_pages; i += step) {
+        const int b = owner(ps, (int32_t)i);
+        const int32_t old = (a.cached[b] + KV4_PAGE - 1) / KV4_PAGE;
+        a.table[b * a.table_stride + old + i - ps[b]] = a.free_pages[i];
+    }
+}
+
+hipError_t enqueue_kv4_tables(const Kv4Tables &a, hipStream_t s)
+{
+    const int64_t items = std::max<int64_t>(a.n_rows, a.n_seqs + 1);
+    const int grid = (int)std::min<int64_t>((items + 1023) / 1024, 256);
+    hipLaunchKernelGGL(k_kv4_tables, dim3(grid), dim3(1024), 0, s, a);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// k_qk_norm_rope
+// ---------------------------------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_mov64(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// sums over L = 8 or 16 neighbouring lanes, the same in each
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v += dpp_mov<0xB1>(v);
+    v += dpp_mov<0x4E>(v);
+    v += dpp_mov<0x141>(v);
+    if constexpr (L == 16) v += dpp_mov<0x140>(v);
+    return v;
+}
+template <int L>
+__device__ __forceinline__ double lanes_sum(double v)
+{
+    v += dpp_mov64<0xB1>(v);
+    v += dpp_mov64<0x4E>(v);
+    v += dpp_mov64<0x141>(v);
+    if constexpr (L == 16) v += dpp_mov64<0x140>(v);
+    return v;
+}
+
+// One lane's part of a head: columns 4j .. 4j+3 and, D / 2 further, the ones
+// they are rotated with.
+template <class F>
+struct Head {
+    F a[4], b[4];
+};
+
+// The norm over the head's lanes and the rotation.  F float for rows that
+// leave in their own type, double for keys that are quantised: a code is
+// decided where a value lies between two borders, and sums in another order
+// must not move it.
+template <class F, int L>
+__device__ __forceinline__ void norm_rope(Head<F> &x, bool norm, f32x4 ga, f32x4 gb, float eps, bool rope, f32x4 c, f32x4 s)
+{
+    if (norm) {
+        F ss = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+        ss = lanes_sum<L>(ss);
+        const F r = F(1) / (F)sqrt(ss * F(1.0 / (8 * L)) + (F)eps);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x.a[i] = x.a[i] * r * (F)ga[i];
+            x.b[i] = x.b[i] * r * (F)gb[i];
+        }
+    }
+    if (!rope) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const F a = x.a[i], b = x.b[i];
+        x.a[i] = a * (F)c[i] - b * (F)s[i];
+        x.b[i] = b * (F)c[i] + a * (F)s[i];
+    }
+}
+
+// Codes and scale of 32 values, four in each of eight neighbouring lanes: the
+// step is -1/8 of the value of largest magnitude, rounded to f16 and then to
+// 8 significant bits; the nearest step's number, halves to even, plus 8.  The
+// quotient is a product with the reciprocal except next to a half, where only
+// the division says on which side it lies.
+__device__ __forceinline__ uint32_t quantise(const double (&x)[4], uint16_t &scale)
+{
+    double v[4], hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = fmin(fmax(x[i], -65280.0), 65280.0);
+    hi = fmax(fmax(v[0], v[1]), fmax(v[2], v[3]));
+    lo = fmin(fmin(v[0], v[1]), fmin(v[2], v[3]));
+    hi = fmax(hi, dpp_mov64<0xB1>(hi)), lo = fmin(lo, dpp_mov64<0xB1>(lo));
+    hi = fmax(hi, dpp_mov64<0x4E>(hi)), lo = fmin(lo, dpp_mov64<0x4E>(lo));
+    hi = fmax(hi, dpp_mov64<0x141>(hi)), lo = fmin(lo, dpp_mov64<0x141>(lo));
+    const _Float16 h = (_Float16)(float)((hi >= -lo ? hi : lo) * -0.125);
+    scale = (uint16_t)((__builtin_bit_cast(uint16_t, h) + 4) & 0xFFF8);
+    const double d = (double)(float)__builtin_bit_cast(_Float16, scale);
+    const double inv = d != 0.0 ? 1.0 / d : 0.0;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double q = v[i] * inv;
+        double r = rint(q);
+        if (fabs(fabs(q - r) - 0.5) < 1e-9) r = rint(v[i] / d);
+        codes |= (uint32_t)(int)fmin(fmax(r + 8.0, 0.0), 15.0) << (4 * i);
+    }
+    return codes;
+}
+
+// D / 8 lanes take one row's query heads of one kv head, that kv head's key
+// and, with a cache, its value: the angles are loaded once for all of them.
+// Bound by memory: rows in, q out and 4.5 bits a value into the pages.
+template <class T, int D, bool STORE>
+__global__ void __launch_bounds__(256)
+k_qk_norm_rope(QkNormRope a)
+{
+    constexpr int L = D / 8;
+    const int j = threadIdx.x % L;
+    const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (item >= (int64_t)a.rows * a.kv_heads) return;
+    const int row = (int)(item / a.kv_heads), hk = (int)(item % a.kv_heads);
+    const int32_t pos = a.positions ? a.positions[row] : 0;
+    if (pos < 0) return;
+    const bool vec = a.vec;
+    const int at = 4 * j, up = D / 2 + 4 * j;    // a lane's columns
+
+    const T *kp = (const T *)a.k + row * a.k_stride + hk * D;
+    const f32x4 ka = load4(kp + at, vec), kb = load4(kp + up, vec);
+    f32x4 va{}, vb{};
+    if constexpr (STORE) {
+        const T *vp = (const T *)a.v + row * a.v_stride + hk * D;
+        va = load4(vp + at, vec), vb = load4(vp + up, vec);
+    }
+    f32x4 c{}, s{};
+    if (a.positions) {
+        if (pos < a.max_pos) {
+            c = load4(a.cos + (int64_t)pos * (D / 2) + at, vec);
+            s = load4(a.sin + (int64_t)pos * (D / 2) + at, vec);
+        } else {
+            c = s = __builtin_nanf("");
+        }
+    }
+
+    f32x4 ga{}, gb{};
+    if (a.q_norm) ga = load4((const _Float16 *)a.q_norm + at, vec), gb = load4((const _Float16 *)a.q_norm + up, vec);
+    for (int g = 0; g < a.group; g++) {
+        const int h = hk * a.group + g;
+        const T *qp = (const T *)a.q + row * a.q_stride + h * D;
+        const f32x4 qa = load4(qp + at, vec), qb = load4(qp + up, vec);
+        Head<float> x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.a[i] = qa[i], x.b[i] = qb[i];
+        norm_rope<float, L>(x, a.q_norm, ga, gb, a.eps, a.positions, c, s);
+        T *qo = (T *)a.q_out + row * a.q_out_stride + h * D;
+        store4(qo + at, f32x4{x.a[0], x.a[1], x.a[2], x.a[3]}, vec);
+        store4(qo + up, f32x4{x.b[0], x.b[1], x.b[2], x.b[3]}, vec);
+    }
+
+    if (a.k_norm) ga = load4((const _Float16 *)a.k_norm + at, vec), gb = load4((const _Float16 *)a.k_norm + up, vec);
+    using F = typename std::conditional<STORE, double, float>::type;
+    Head<F> x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x.a[i] = ka[i], x.b[i] = kb[i];
+    norm_rope<F, L>(x, a.k_norm, ga, gb, a.eps, a.positions, c, s);
+    if (a.k_out) {
+        T *ko = (T *)a.k_out + row * a.k_out_stride + hk * D;
+        store4(ko + at, f32x4{(float)x.a[0], (float)x.a[1], (float)x.a[2], (float)x.a[3]}, vec);
+        store4(ko + up, f32x4{(float)x.b[0], (float)x.b[1], (float)x.b[2], (float)x.b[3]}, vec);
+    }
+    if constexpr (STORE) {
+        bool nan = false;
+        double y[4], z[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            nan |= x.a[i] != x.a[i] || x.b[i] != x.b[i] || va[i] != va[i] || vb[i] != vb[i];
+            y[i] = va[i], z[i] = vb[i];
+        }
+        // any lane of the head
+        const uint64_t lanes = ((1ull << L) - 1) << (threadIdx.x % 64 / L * L);
+        nan = (__ballot(nan) & lanes) != 0;
+        uint16_t s0, s1, s2, s3;
+        const uint32_t k0 = quantise(x.a, s0), k1 = quantise(x.b, s1);
+        const uint32_t v0 = quantise(y, s2), v1 = quantise(z, s3);
+        const int64_t slot = a.slots[row];
+        if (slot < 0 || slot >= a.cache.n_pages * KV4_PAGE) return;
+        uint8_t *blk = a.cache.base + slot / KV4_PAGE * a.cache.stride + (int64_t)hk * kv4_block(D);
+        const int p = (int)(slot % KV4_PAGE);
+        *(uint16_t *)(blk + kv4_k_at(D, p) + 2 * j) = (uint16_t)k0;
+        *(uint16_t *)(blk + kv4_k_at(D, p) + D / 4 + 2 * j) = (uint16_t)k1;
+        *(uint16_t *)(blk + kv4_v_at(D, p, j)) = (uint16_t)v0;
+        *(uint16_t *)(blk + kv4_v_at(D, p, j + D / 8)) = (uint16_t)v1;
+        if (j % 8 == 0) {
+            *(uint16_t *)(blk + kv4_ks_at(D, p, j / 8)) = nan ? 0x7E00 : s0;
+            *(uint16_t *)(blk + kv4_ks_at(D, p, j / 8 + D / 64)) = nan ? 0x7E00 : s1;
+            *(uint16_t *)(blk + kv4_vs_at(D, p, j / 8)) = nan ? 0 : s2;
+            *(uint16_t *)(blk + kv4_vs_at(D, p, j / 8 + D / 64)) = nan ? 0 : s3;
+        }
+    }
+}
+
+template <class T, int D>
+static hipError_t launch_qk(const QkNormRope &a, bool store, hipStream_t s)
+{
+    const int64_t groups = (int64_t)a.rows * a.kv_heads, per = 256 / (D / 8);
+    const dim3 grid((unsigned)((groups + per - 1) / per));
+    if (store)
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, true>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+// F<T, D>::go for an element type and head width that the caller has checked
+#define KV4_TYPED(dtype, D, call)                                            \
+    do {                                                                     \
+        if ((D) == 64) {                                                     \
+            if ((dtype) == QTTS_F32) { using T = float; constexpr int HD = 64; return call; }      \
+            if ((dtype) == QTTS_F16) { using T = _Float16; constexpr int HD = 64; return call; }   \
+            using T = __bf16; constexpr int HD = 64; return call;            \
+        }                                                                    \
+        if ((dtype) == QTTS_F32) { using T = float; constexpr int HD = 128; return call; }         \
+        if ((dtype) == QTTS_F16) { using T = _Float16; constexpr int HD = 128; return call; }      \
+        using T = __bf16; constexpr int HD = 128; return call;               \
+    } while (0)
+
+hipError_t enqueue_qk_norm_rope(const QkNormRope &a, int dtype, int D, bool store, hipStream_t s)
+{
+    KV4_TYPED(dtype, D, (launch_qk<T, HD>(a, store, s)));
+}
+
+// ---------------------------------------------------------------------------
+// k_kv4_gather
+// ---------------------------------------------------------------------------
+
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+k_kv4_gather(Kv4Pages c, const int64_t *slots, int n, T *K, T *V)
+{
+    constexpr int L = D / 4;                     // lanes of a head, four columns each
+    const int u = threadIdx.x % L;
+    const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (item >= (int64_t)n * c.heads) return;
+    const int i = (int)(item / c.heads), h = (int)(item % c.heads), g = u / 8;
+    const int64_t slot = slots[i];
+    uint32_t kc = 0x8888, vc = 0x8888;
+    float ks = 0.0f, vs = 0.0f;
+    if (slot >= 0 && slot < c.n_pages * KV4_PAGE) {
+        const uint8_t *blk = c.base + slot / KV4_PAGE * c.stride + (int64_t)h * kv4_block(D);
+        const int p = (int)(slot % KV4_PAGE);
+        kc = *(const uint16_t *)(blk + kv4_k_at(D, p) + 2 * u);
+        vc = *(const uint16_t *)(blk + kv4_v_at(D, p, u));
+        ks = h2f(*(const uint16_t *)(blk + kv4_ks_at(D, p, g)));
+        vs = h2f(*(const uint16_t *)(blk + kv4_vs_at(D, p, g)));
+    }
+    f32x4 k, v;
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        k[b] = (float)((int)(kc >> (4 * b) & 15) - 8) * ks;
+        v[b] = (float)((int)(vc >> (4 * b) & 15) - 8) * vs;
+    }
+    const int64_t at = item * D + 4 * u;
+    if (K) store4(K + at, k, true);
+    if (V) store4(V + at, v, true);
+}
+
+template <class T, int D>
+static hipError_t launch_gather(const Kv4Pages &c, const int64_t *slots, int n, void *K, void *V, hipStream_t s)
+{
+    const int64_t items = (int64_t)n * c.heads, per = 256 / (D / 4);
+    hipLaunchKernelGGL((k_kv4_gather<T, D>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, c, slots, n,
+                       (T *)K, (T *)V);
+    return hipGetLastError();
+}
+
+hipError_t enqueue_kv4_gather(const Kv4Pages &c, int D, const int64_t *slots, int n, int dtype, void *K, void *V, hipStream_t s)
+{
+    KV4_TYPED(dtype, D, (launch_gather<T, HD>(c, slots, n, K, V, s)));
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float max_xor32(float v)
+{
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    unsigned w;
+    asm volatile("" : "=v"(w) : "0"(u));
+    const auto r = __builtin_amdgcn_permlane32_swap(u, w, false, false);
+    unsigned a = r[0], b = r[1];
+    asm volatile("" : "+v"(a), "+v"(b));
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+__device__ __forceinline__ float max_xor16(float v)
+{
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    unsigned w;
+    asm volatile("" : "=v"(w) : "0"(u));
+    const auto r = __builtin_amdgcn_permlane16_swap(u, w, false, false);
+    unsigned a = r[0], b = r[1];
+    asm volatile("" : "+v"(a), "+v"(b));
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+__device__ __forceinline__ float add_xor16(float v)
+{
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    unsigned w;
+    asm volatile("" : "=v"(w) : "0"(u));
+    const auto r = __builtin_amdgcn_permlane16_swap(u, w, false, false);
+    return swap_pair_sum(r[0], r[1]);
+}
+
+__device__ __forceinline__ h16x2 as_h2(uint32_t u) { return __builtin_bit_cast(h16x2, u); }
+__device__ __forceinline__ uint32_t as_u(h16x2 h) { return __builtin_bit_cast(uint32_t, h); }
+
+// Eight codes (four bits at 0, 4, 8 and 12 of each half of w) times scales, as
+// f16 pairs: out[n] = (code n of the low half, code n of the high half).  A
+// code under 0x6400 is the f16 1024 + code, four bits further up 1024 + 16
+// code; the subtraction, the factor 1/16 and the product with a scale of 8
+// significant bits are all exact.
+__device__ __forceinline__ void unpack8(uint32_t w, const h16x2 scale, uint32_t (&out)[4])
+{
+    const h16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const h16x2 m0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, m1 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const uint32_t w8 = w >> 8;
+    const h16x2 c0 = as_h2((w & 0x000F000Fu) | 0x64006400u) + m0;
+    const h16x2 c1 = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, m1);
+    const h16x2 c2 = as_h2((w8 & 0x000F000Fu) | 0x64006400u) + m0;
+    const h16x2 c3 = __builtin_elementwise_fma(as_h2((w8 & 0x00F000F0u) | 0x64006400u), sixteenth, m1);
+    out[0] = as_u(c0 * scale);
+    out[1] = as_u(c1 * scale);
+    out[2] = as_u(c2 * scale);
+    out[3] = as_u(c3 * scale);
+}
+
+__device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __builtin_bit_cast(half8, u32x4{a, b, c, d});
+}
+
+// What a tile of W columns is: its sequence's rows r0 .. r0 + n - 1 at the end
+// of `len` positions, its first column cb of n * group.
+struct AttnTile {
+    int b, r0, n, len, cb, ncols;
+};
+
+// The tile with number ti, found by the whole wave: each round, 64 lanes look
+// at 64 evenly spaced sequences (one load of latency for 64 sequences, two
+// for 4096).  False where no tile has this number, and for row sums that
+// are none.
+__device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnTile &t)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, cnt = a.n_seqs;
+    while (cnt > 1) {
+        const int step = (cnt + 63) / 64, i = lane * step;
+        const bool in = i < cnt && kv4_first_tile(min(max(a.row_start[lo + i], 0), a.rows), a.group, lo + i, W) <= ti;
+        const uint64_t m = __ballot(in);
+        const int last = m ? 63 - __clzll(m) : 0;
+        lo += last * step;
+        cnt = min(step, cnt - last * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    t.b = lo;
+    t.r0 = a.row_start[lo];
+    const int r1 = a.row_start[lo + 1];
+    t.len = a.lengths[lo];
+    if (t.r0 < 0 || r1 > a.rows || r1 <= t.r0 || t.len < 0 || t.len > INT32_MAX - KV4_PAGE) return false;
+    t.n = r1 - t.r0;
+    t.ncols = t.n * a.group;
+    const int64_t rel = ti - kv4_first_tile(t.r0, a.group, lo, W);
+    if (rel < 0 || rel * W >= t.ncols) return false;
+    t.cb = (int)rel * W;
+    return true;
+}
+
+// The last position that a column sees is len - n + row; keys [lo, hi) are
+// what the tile's columns see at all.
+__device__ __forceinline__ void tile_keys(const AttnTile &t, int group, int window, int W, int &minpos, int &maxpos,
+                                          int &lo, int &hi)
+{
+    minpos = t.len - t.n + t.cb / group;
+    maxpos = t.len - t.n + min(t.cb + W - 1, t.ncols - 1) / group;
+    hi = maxpos + 1;
+    lo = window ? max(0, minpos - window + 1) : 0;
+}
+
+// One page's block as a wave holds it: lane l = (r, kg) = (l % 16, l / 16) has
+// of K rows 4r + t (t = 0..3) the D / 4 columns from kg D / 4, of V positions
+// 16 kg .. 16 kg + 15 of the D / 16 columns from r D / 16, and their scales.
+template <int D>
+struct PageRegs {
+    uint32_t k[4][D / 32], v[4][D / 32], ks[2], vs[8];
+};
+
+template <int D>
+__device__ __forceinline__ void load_words(uint32_t *out, const uint8_t *p)
+{
+    if constexpr (D == 128) {
+        const u32x4 w = *(const u32x4 *)p;
+        out[0] = w.x, out[1] = w.y, out[2] = w.z, out[3] = w.w;
+    } else {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 w = *(const u32x2 *)p;
+        out[0] = w.x, out[1] = w.y;
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void load_page(PageRegs<D> &g, const uint8_t *blk, int r, int kg)
+{
+#pragma unroll
+    for (int t = 0; t < 4; t++) load_words<D>(g.k[t], blk + kv4_k_at(D, 4 * r + t) + kg * (D / 8));
+    const uint2 ks = *(const uint2 *)(blk + kv4_ks_at(D, 4 * r, kg * (D / 4) / 32));
+    g.ks[0] = ks.x, g.ks[1] = ks.y;
+#pragma unroll
+    for (int q = 0; q < 4; q++) load_words<D>(g.v[q], blk + kv4_v_at(D, 16 * kg + 4 * q, r * (D / 64)));
+    const u32x4 *vs = (const u32x4 *)(blk + kv4_vs_at(D, 16 * kg, r * (D / 16) / 32));
+    const u32x4 v0 = vs[0], v1 = vs[1];
+    g.vs[0] = v0.x, g.vs[1] = v0.y, g.vs[2] = v0.z, g.vs[3] = v0.w;
+    g.vs[4] = v1.x, g.vs[5] = v1.y, g.vs[6] = v1.z, g.vs[7] = v1.w;
+}
+
+// A column's query as the second operand of K q: its D / 4 values from kg D /
+// 4, eight to a step in the order in which unpack8 leaves K's.  Values are
+// first scaled by the power of two that puts the row's largest near 2^14
+// (undone in `unit`): a bf16 or f32 row of any range fits f16; f32 keeps 22
+// bits in two parts.
+template <class T, int D>
+struct Query {
+    static constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
+    half8 f[PARTS][D / 32];
+};
+
+template <class T, int D>
+__device__ __forceinline__ float load_query(Query<T, D> &q, const T *p, bool valid, bool vec)
+{
+    f32x4 x[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) x[i] = valid ? load4(p + 4 * i, vec) : f32x4{0, 0, 0, 0};
+    float unit = 1.0f;
+    if constexpr (!std::is_same<T, _Float16>::value) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[i][e]));
+        mx = max_xor32(max_xor16(mx));
+        const int sh = range_shift(mx);
+        const float up = ldexpf(1.0f, sh);
+        unit = ldexpf(1.0f, -sh);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) x[i] *= up;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) {
+        const f32x4 lo = x[2 * j], hi = x[2 * j + 1];
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) split_f16_pair<true>(lo[n], hi[n], h[n], l[n]);
+        q.f[0][j] = as_half8(h[0], h[1], h[2], h[3]);
+        if constexpr (Query<T, D>::PARTS == 2) q.f[1][j] = as_half8(l[0], l[1], l[2], l[3]);
+    }
+    return unit;
+}
+
+// Running state of 16 columns in a wave: lane (m, kg) holds column m's maximum
+// (in units of log2), its own share of the sum, and rows D/16 (4 kg + e) + i of
+// the output as o[i][e].  Probabilities are kept times 2^14, where f16 holds
+// the small ones too; sums and outputs carry the factor until they are divided.
+template <int D>
+struct Running {
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[D / 16] = {};
+};
+
+// One page: scores of 64 keys (lane (m, kg): keys 16 kg + 4 i + t), the running
+// softmax, and P V on the same lanes, with no exchange between lanes but the
+// maximum's.
+template <class T, int D>
+__device__ __forceinline__ void page_step(Running<D> &s, const PageRegs<D> &g, const Query<T, D> &q, float unit,
+                                          bool edge, int key0, int pos, int window, int len, int kg)
+{
+    constexpr int PARTS = Query<T, D>::PARTS;
+    f32x4 x[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const uint32_t sc = g.ks[t / 2];
+        const uint32_t both = t % 2 ? (sc >> 16) | (sc & 0xFFFF0000u) : (sc & 0xFFFFu) | (sc << 16);
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+            uint32_t a[4];
+            unpack8(g.k[t][j], as_h2(both), a);
+            const half8 k8 = as_half8(a[0], a[1], a[2], a[3]);
+            if constexpr (PARTS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q.f[1][j], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q.f[0][j], acc, 0, 0, 0);
+        }
+        x[t] = acc;
+    }
+    uint32_t vs[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) vs[i] = g.vs[i];
+    if (edge) {
+        // keys that a column does not see; values past the sequence's end,
+        // which may hold anything, count as zero (0 * NaN is not 0)
+        const int first = key0 + 16 * kg;
+        const int low = window ? pos - window : -1;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = first + 4 * i + t;
+                if (key > pos || key <= low) x[t][i] = -INFINITY;
+            }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int left = len - (first + 2 * i);
+            vs[i] = left <= 0 ? 0u : left == 1 ? vs[i] & 0xFFFFu : vs[i];
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; t++) top = fmaxf(top, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+    top = max_xor32(max_xor16(top)) * unit;
+    const float m = fmaxf(s.m, top);
+    if (__any(m > s.m)) {
+        const float f = m > s.m ? __builtin_amdgcn_exp2f(s.m - m) : 1.0f;   // exp2(-inf) = 0 at the first page
+        s.l *= f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) s.o[i] *= f;
+        s.m = m;
+    }
+    const float off = m == -INFINITY ? 0.0f : 14.0f - m;
+    float p[16];                     // key 16 kg + 4 i + t at 4 i + t
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) p[4 * i + t] = __builtin_amdgcn_exp2f(fmaf(x[t][i], unit, off));
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum += p[i];
+    s.l += sum;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) split_f16_pair<true>(p[8 * u + 2 * n], p[8 * u + 2 * n + 1], ph[n], pl[n]);
+        const half8 p8 = as_half8(ph[0], ph[1], ph[2], ph[3]);
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) {       // units of four columns
+            uint32_t a[4][4];
+#pragma unroll
+            for (int h = 0; h < 4; h++) unpack8(g.v[2 * u + h / 2][2 * c + h % 2], as_h2(vs[4 * u + h]), a[h]);
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const half8 v8 = as_half8(a[0][n], a[1][n], a[2][n], a[3][n]);
+                f32x4 &o = s.o[4 * c + n];
+                if constexpr (PARTS == 2)
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, as_half8(pl[0], pl[1], pl[2], pl[3]), o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p8, o, 0, 0, 0);
+            }
+        }
+    }
+}
+
+// Attention of 16 columns of one kv head over a share of the tile's pages, the
+// four waves taking them in turn and joining through LDS.
+template <class T, int D>
+__global__ void __launch_bounds__(256, 2)
+k_kv4_attn(Kv4Attn a)
+{
+    constexpr int W = KV4_W, LD = D + 4;
+    __shared__ float so[4][W][LD], sm[4][W], sl[4][W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, kg = lane >> 4;
+    const int ti = blockIdx.x, sp = blockIdx.y, hk = blockIdx.z;
+    AttnTile t;
+    if (!find_tile(a, ti, W, t)) return;
+    int minpos, maxpos, lo, hi;
+    tile_keys(t, a.group, a.window, W, minpos, maxpos, lo, hi);
+    const int pg0 = lo / KV4_PAGE, pg1 = min((hi + KV4_PAGE - 1) / KV4_PAGE, a.max_pages);
+    const int pages = hi > lo ? max(pg1 - pg0, 0) : 0;
+    const int pb = pg0 + (int)((int64_t)pages * sp / a.splits), pe = pg0 + (int)((int64_t)pages * (sp + 1) / a.splits);
+
+    const int cc = t.cb + r, row = cc / a.group;
+    const bool valid = cc < t.ncols;
+    const int pos = valid ? t.len - t.n + row : -1;
+    Query<T, D> q;
+    const T *qp = (const T *)a.q + (t.r0 + row) * a.q_stride + (hk * a.group + cc % a.group) * D + kg * (D / 4);
+    float unit = load_query<T, D>(q, qp, valid, a.vec) * (a.scale * 1.44269504088896341f);
+    if (a.scale < 0.0f) {            // the running maximum is taken before the factor
+        unit = -unit;
+#pragma unroll
+        for (int i = 0; i < Query<T, D>::PARTS; i++)
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) q.f[i][j] = -q.f[i][j];
+    }
+
+    unit = fmaxf(unit, 1.2e-38f);    // 0 * -inf would be NaN
+    Running<D> s;
+    bool poisoned = pos >= (int64_t)a.max_pages * KV4_PAGE;   // sees a page that the table has no column for
+    const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
+    for (int base = pb + wave; base < pe; base += 256) {
+        // 64 of this wave's pages: one id a lane
+        const int mine = base + 4 * lane;
+        const int id = mine < pe ? table[mine] : -1;
+        const int count = min(64, (pe - base + 3) / 4);
+        for (int i = 0; i < count; i++) {
+            const int page = base + 4 * i;
+            const int pid = __builtin_amdgcn_readlane(id, i);
+            const bool bad = pid < 0 || pid >= a.cache.n_pages;
+            if (bad) {               // what sees this page is NaN
+                const int first = page * KV4_PAGE;
+                poisoned |= pos >= first && (!a.window || pos - a.window < first + KV4_PAGE - 1);
+                continue;
+            }
+            PageRegs<D> g;
+            load_page<D>(g, a.cache.base + pid * a.cache.stride + (int64_t)hk * kv4_block(D), r, kg);
+            const int key0 = page * KV4_PAGE;
+            const bool edge = key0 + KV4_PAGE - 1 > minpos || (a.window && key0 <= maxpos - a.window);
+            page_step<T, D>(s, g, q, unit, edge, key0, pos, a.window, t.len, kg);
+        }
+    }
+    s.l = add_xor32(add_xor16(s.l));
+    if (poisoned) s.l = __builtin_nanf("");
+    if (kg == 0) sm[wave][r] = s.m, sl[wave][r] = s.l;
+    __syncthreads();
+    float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    const float f = s.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.m - M);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4)
+            *(f32x4 *)&so[wave][r][D / 16 * (4 * kg + e) + i] =
+                f32x4{s.o[i][e], s.o[i + 1][e], s.o[i + 2][e], s.o[i + 3][e]} * f;
+    __syncthreads();
+    const int64_t pi = ((int64_t)ti * a.cache.heads + hk) * a.splits + sp;
+    for (int i = threadIdx.x; i < W * D / 4; i += 256) {
+        const int c = i / (D / 4), d = i % (D / 4) * 4, col = t.cb + c;
+        if (col >= t.ncols) break;
+        f32x4 o = {0, 0, 0, 0};
+        float l = 0.0f;
+        const float Mc = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            o += *(const f32x4 *)&so[w][c][d];
+            l += sm[w][c] == -INFINITY ? 0.0f * sl[w][c] : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - Mc);
+        }
+        if (a.splits > 1) {
+            if (d == 0) a.part[pi * 32 + c] = Mc, a.part[pi * 32 + 16 + c] = l;
+            *(f32x4 *)(a.part + a.part_rows + (pi * W + c) * D + d) = o;
+        } else {
+            // a column that saw nothing has l = 0
+            store4((T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + d,
+                   l == 0.0f ? f32x4{0, 0, 0, 0} : o / l, a.vec);
+        }
+    }
+}
+
+// The splits of one column joined: weights 2^(m - M), then the rows' weighted
+// sum, 256 / (D / 4) of them at a time.
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+k_kv4_attn_join(Kv4Attn a)
+{
+    constexpr int L = D / 4, ROWS = 256 / L;
+    __shared__ float w[64];
+    __shared__ f32x4 so[ROWS][L];
+    const int ti = blockIdx.x, c = blockIdx.y, hk = blockIdx.z, lane = threadIdx.x & 63;
+    AttnTile t;
+    if (!find_tile(a, ti, KV4_W, t)) return;
+    const int col = t.cb + c;
+    if (col >= t.ncols) return;
+    const int64_t p0 = ((int64_t)ti * a.cache.heads + hk) * a.splits;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < a.splits) m = a.part[(p0 + lane) * 32 + c], l = a.part[(p0 + lane) * 32 + 16 + c];
+    const float M = wave_max_dpp(m);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    const float sum = wave_sum_dpp(l * f);
+    if (threadIdx.x < 64) w[lane] = f;
+    __syncthreads();
+    const int i = threadIdx.x % L, g = threadIdx.x / L;
+    f32x4 o = {0, 0, 0, 0};
+    for (int s = g; s < a.splits; s += ROWS)
+        o += *(const f32x4 *)(a.part + a.part_rows + ((p0 + s) * KV4_W + c) * D + 4 * i) * w[s];
+    so[g][i] = o;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int k = 1; k < ROWS; k++) o += so[k][i];
+    store4((T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + 4 * i,
+           sum == 0.0f ? f32x4{0, 0, 0, 0} : o / sum, a.vec);
+}
+
+// Tiles there can be: the number after the last sequence's last.
+static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return kv4_first_tile(rows, group, n_seqs, W); }
+
+// Shares that the pages of each tile are cut into: enough workgroups to fill
+// the card, at least a page for each of their waves.
+int kv4_attn_splits(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
+{
+    const int64_t items = attn_tiles(rows, n_seqs, group, KV4_W) * kv_heads;
+    int64_t pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
+    if (window) pages = std::min<int64_t>(pages, (window + KV4_W - 2) / KV4_PAGE + 2);
+    const int64_t want = std::min((1024 + items - 1) / std::max<int64_t>(items, 1), (pages + 3) / 4);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
+}
+
+template <class T, int D>
+static hipError_t launch_attn(const Kv4Attn &a, hipStream_t s)
+{
+    const unsigned tiles = (unsigned)attn_tiles(a.rows, a.n_seqs, a.group, KV4_W);
+    hipLaunchKernelGGL((k_kv4_attn<T, D>), dim3(tiles, a.splits, a.cache.heads), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    hipLaunchKernelGGL((k_kv4_attn_join<T, D>), dim3(tiles, KV4_W, a.cache.heads), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, hipStream_t s)
+{
+    KV4_TYPED(dtype, D, (launch_attn<T, HD>(a, s)));
+}
+
+}  // namespace qtts

@@ -4,6 +4,7 @@
 #include "../../include/qtts.h"
 #include "qtts_device.h"
 #include "qtts_kernels.h"
+#include "qtts_kv4.h"
 
 #include <hip/hip_runtime.h>
 
@@ -1874,6 +1875,277 @@ extern "C" int qtts_prefill_custom_voice(qtts_ctx *c, const uint32_t *text_token
     RCHK(finish(c));
     *position_out = icl_rows ? 9 + n_icl : (n_text > 0 ? 10 : 9);
     return QTTS_OK;
+}
+
+// ---------------------------------------------------------------------------
+// many sequences over a 4-bit cache: argument checks and launches (device
+// pointers, the caller's stream, nothing allocated)
+// ---------------------------------------------------------------------------
+
+// The caller's current device, put back where the context's is another one.
+struct DeviceGuard {
+    int was = -1;
+    explicit DeviceGuard(int device)
+    {
+        int now = device;
+        if (hipGetDevice(&now) == hipSuccess && now != device) {
+            was = now;
+            hipSetDevice(device);
+        }
+    }
+    ~DeviceGuard() { if (was >= 0) hipSetDevice(was); }
+};
+
+static bool kv4_aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+static int64_t kv4_size(int dtype) { return dtype == QTTS_F32 ? 4 : 2; }
+
+// Rows of `width` bytes every `stride` bytes: whether two such sets share a
+// byte.  Interleaved columns of one buffer (q, k and v of a joint linear map)
+// do not.
+struct Rows {
+    const void *p;
+    int64_t n, stride, width;
+    uintptr_t begin() const { return (uintptr_t)p; }
+    uintptr_t end() const { return n > 0 ? begin() + (uintptr_t)((n - 1) * stride + width) : begin(); }
+};
+static bool rows_clash(const Rows &a, const Rows &b)
+{
+    if (!a.p || !b.p || a.begin() >= b.end() || b.begin() >= a.end()) return false;
+    if (a.stride != b.stride || a.stride <= 0) return true;
+    const Rows &lo = a.begin() <= b.begin() ? a : b, &hi = a.begin() <= b.begin() ? b : a;
+    const int64_t off = (int64_t)((hi.begin() - lo.begin()) % (uintptr_t)a.stride);
+    return off < lo.width || off + hi.width > a.stride;
+}
+static Rows flat(const void *p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+
+static int check_kv4(qtts_ctx *c, const qtts_kv4 *k)
+{
+    if (!k || !k->base) return fail(c, QTTS_ERR_INVALID, "null cache");
+    if (k->head_dim != 64 && k->head_dim != 128)
+        return fail(c, QTTS_ERR_UNSUPPORTED, "a 4-bit cache holds heads of 64 or 128, not %d", k->head_dim);
+    if (k->n_kv_heads < 1 || k->n_kv_heads > 65535) return fail(c, QTTS_ERR_INVALID, "%d kv heads", k->n_kv_heads);
+    if (k->n_pages < 1 || k->n_pages > INT32_MAX) return fail(c, QTTS_ERR_INVALID, "%lld pages", (long long)k->n_pages);
+    if (k->page_stride < (int64_t)k->n_kv_heads * kv4_block(k->head_dim) || k->page_stride % 16 ||
+        k->page_stride > ((int64_t)1 << 31) || !kv4_aligned(k->base, 16))
+        return fail(c, QTTS_ERR_INVALID, "cache pages must be 16-byte aligned and at least %lld bytes apart (stride %lld)",
+                    (long long)k->n_kv_heads * kv4_block(k->head_dim), (long long)k->page_stride);
+    return QTTS_OK;
+}
+static Kv4Pages pages_of(const qtts_kv4 &k) { return {(uint8_t *)k.base, k.n_pages, k.page_stride, k.n_kv_heads}; }
+static Rows rows_of(const qtts_kv4 &k)
+{
+    return {k.base, k.n_pages, k.page_stride, (int64_t)k.n_kv_heads * kv4_block(k.head_dim)};
+}
+
+static int check_dtype(qtts_ctx *c, int dtype)
+{
+    if (dtype != QTTS_F32 && dtype != QTTS_F16 && dtype != QTTS_BF16) return fail(c, QTTS_ERR_UNSUPPORTED, "element type %d", dtype);
+    return QTTS_OK;
+}
+
+// rows [rows][heads * head_dim] of `dtype`, `stride` elements apart
+static int check_rows(qtts_ctx *c, const char *name, const void *p, int64_t rows, int64_t heads, int D, int64_t stride, int dtype)
+{
+    if (!p && rows) return fail(c, QTTS_ERR_INVALID, "%s is null", name);
+    if (!kv4_aligned(p, (size_t)kv4_size(dtype))) return fail(c, QTTS_ERR_INVALID, "%s is not aligned to its element type", name);
+    if (stride < heads * D || stride > INT32_MAX)
+        return fail(c, QTTS_ERR_INVALID, "%s: row stride %lld below %lld", name, (long long)stride, (long long)(heads * D));
+    return QTTS_OK;
+}
+
+// four elements of each row can move at once
+static bool moves4(const void *p, int64_t stride, int dtype)
+{
+    return !p || (kv4_aligned(p, (size_t)(4 * kv4_size(dtype))) && stride % 4 == 0);
+}
+
+static int kv4_done(qtts_ctx *c, hipError_t e)
+{
+    if (e != hipSuccess) return fail(c, QTTS_ERR_HIP, "launch: %s", hipGetErrorString(e));
+    return QTTS_OK;
+}
+
+extern "C" int qtts_kv4_tables(qtts_ctx *c, const qtts_kv4_tables_args *a, void *stream, int flags)
+{
+    if (!a || (!c && !(flags & QTTS_CHECK_ONLY))) return QTTS_ERR_INVALID;
+    if (a->n_seqs < 0 || a->n_rows < 0 || a->n_free < 0 || a->max_pages < 0 || a->table_stride < a->max_pages)
+        return fail(c, QTTS_ERR_INVALID, "negative size, or a table row shorter than its columns");
+    if (a->n_seqs > KV4_MAX_SEQS) return fail(c, QTTS_ERR_CAPACITY, "at most %d sequences", KV4_MAX_SEQS);
+    if (a->n_rows > INT32_MAX || a->n_free > INT32_MAX || a->max_pages > INT32_MAX / KV4_PAGE - 2 || a->table_stride > INT32_MAX)
+        return fail(c, QTTS_ERR_CAPACITY, "rows, pages and positions are counted in 32 bits");
+    if (!a->row_start || !a->status || (a->n_seqs && (!a->cached || !a->fresh || !a->lengths)) ||
+        (a->n_seqs && a->max_pages && !a->table) || (a->n_free && !a->free_pages) || (a->n_rows && (!a->positions || !a->slots)))
+        return fail(c, QTTS_ERR_INVALID, "null array");
+    for (const void *p : {(const void *)a->cached, (const void *)a->fresh, (const void *)a->free_pages, (const void *)a->table,
+                          (const void *)a->row_start, (const void *)a->lengths, (const void *)a->positions, (const void *)a->status})
+        if (!kv4_aligned(p, 4)) return fail(c, QTTS_ERR_INVALID, "array not aligned to its element type");
+    if (!kv4_aligned(a->slots, 8)) return fail(c, QTTS_ERR_INVALID, "array not aligned to its element type");
+    const Rows r[] = {flat(a->cached, 4LL * a->n_seqs), flat(a->fresh, 4LL * a->n_seqs), flat(a->free_pages, 4 * a->n_free),
+                      {a->table, a->n_seqs, 4 * a->table_stride, 4LL * a->max_pages}, flat(a->row_start, 4LL * (a->n_seqs + 1)),
+                      flat(a->lengths, 4LL * a->n_seqs), flat(a->positions, 4 * a->n_rows), flat(a->slots, 8 * a->n_rows),
+                      flat(a->status, 8)};
+    for (int i = 0; i < 9; i++)
+        for (int j = std::max(i + 1, 3); j < 9; j++)
+            if (rows_clash(r[i], r[j])) return fail(c, QTTS_ERR_INVALID, "an output overlaps another array");
+    if (flags & QTTS_CHECK_ONLY) return QTTS_OK;
+    Kv4Tables k{};
+    k.cached = a->cached, k.fresh = a->fresh, k.free_pages = a->free_pages;
+    k.table = a->table, k.row_start = a->row_start, k.lengths = a->lengths, k.positions = a->positions, k.status = a->status;
+    k.slots = a->slots;
+    k.n_free = a->n_free, k.table_stride = a->table_stride, k.n_rows = a->n_rows;
+    k.n_seqs = a->n_seqs, k.max_pages = a->max_pages;
+    DeviceGuard guard(c->device);
+    return kv4_done(c, enqueue_kv4_tables(k, (hipStream_t)stream));
+}
+
+extern "C" int qtts_qk_norm_rope(qtts_ctx *c, const qtts_qk_norm_rope_args *a, void *stream, int flags)
+{
+    if (!a || (!c && !(flags & QTTS_CHECK_ONLY))) return QTTS_ERR_INVALID;
+    RCHK(check_dtype(c, a->dtype));
+    const int D = a->head_dim, dt = a->dtype;
+    if (D != 64 && D != 128) return fail(c, QTTS_ERR_UNSUPPORTED, "heads of 64 or 128, not %d", D);
+    if (a->rows < 0 || a->n_heads < 1 || a->n_kv_heads < 1 || a->n_heads % a->n_kv_heads)
+        return fail(c, QTTS_ERR_INVALID, "%lld rows, %d / %d heads", (long long)a->rows, a->n_heads, a->n_kv_heads);
+    if (a->rows > (1 << 30) / (int64_t)a->n_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^30 rows x heads a call");
+    RCHK(check_rows(c, "q", a->q, a->rows, a->n_heads, D, a->q_stride, dt));
+    RCHK(check_rows(c, "k", a->k, a->rows, a->n_kv_heads, D, a->k_stride, dt));
+    RCHK(check_rows(c, "q_out", a->q_out, a->rows, a->n_heads, D, a->q_out_stride, dt));
+    if (a->k_out || !a->cache) RCHK(check_rows(c, "k_out", a->k_out, a->rows, a->n_kv_heads, D, a->k_out_stride, dt));
+    if (a->cache) {
+        RCHK(check_kv4(c, a->cache));
+        if (a->cache->n_kv_heads != a->n_kv_heads || a->cache->head_dim != D)
+            return fail(c, QTTS_ERR_INVALID, "the cache holds %d heads of %d", a->cache->n_kv_heads, a->cache->head_dim);
+        RCHK(check_rows(c, "v", a->v, a->rows, a->n_kv_heads, D, a->v_stride, dt));
+        if ((!a->slots && a->rows) || !kv4_aligned(a->slots, 8)) return fail(c, QTTS_ERR_INVALID, "slots null or not aligned");
+    }
+    if (a->positions && (!a->rope_cos || !a->rope_sin || a->rope_max_pos < 1)) return fail(c, QTTS_ERR_INVALID, "rope tables missing");
+    if (!kv4_aligned(a->positions, 4) || !kv4_aligned(a->rope_cos, 4) || !kv4_aligned(a->rope_sin, 4) ||
+        !kv4_aligned(a->q_norm, 2) || !kv4_aligned(a->k_norm, 2))
+        return fail(c, QTTS_ERR_INVALID, "array not aligned to its element type");
+    if (!(a->eps >= 0.0f) || std::isinf(a->eps)) return fail(c, QTTS_ERR_INVALID, "eps %g", a->eps);
+    const int64_t sz = kv4_size(dt), qw = a->n_heads * D * sz, kw = a->n_kv_heads * D * sz;
+    const Rows q = {a->q, a->rows, a->q_stride * sz, qw}, k = {a->k, a->rows, a->k_stride * sz, kw},
+               v = a->cache ? Rows{a->v, a->rows, a->v_stride * sz, kw} : Rows{},
+               qo = {a->q_out, a->rows, a->q_out_stride * sz, qw}, ko = {a->k_out, a->rows, a->k_out_stride * sz, kw},
+               pages = a->cache ? rows_of(*a->cache) : Rows{};
+    const bool q_in_place = a->q_out == a->q && a->q_out_stride == a->q_stride;
+    const bool k_in_place = a->k_out == a->k && a->k_out_stride == a->k_stride;
+    if ((!q_in_place && rows_clash(qo, q)) || (!k_in_place && rows_clash(ko, k)) || rows_clash(qo, k) || rows_clash(qo, v) ||
+        rows_clash(qo, ko) || rows_clash(ko, q) || rows_clash(ko, v) || rows_clash(pages, q) || rows_clash(pages, k) ||
+        rows_clash(pages, v) || rows_clash(pages, qo) || rows_clash(pages, ko))
+        return fail(c, QTTS_ERR_INVALID, "an output overlaps other rows");
+    if ((flags & QTTS_CHECK_ONLY) || a->rows == 0) return QTTS_OK;
+    QkNormRope n{};
+    n.q = a->q, n.k = a->k, n.v = a->v, n.q_out = a->q_out, n.k_out = a->k_out;
+    n.q_stride = a->q_stride, n.k_stride = a->k_stride, n.v_stride = a->v_stride;
+    n.q_out_stride = a->q_out_stride, n.k_out_stride = a->k_out_stride;
+    n.q_norm = a->q_norm, n.k_norm = a->k_norm;
+    n.cos = a->rope_cos, n.sin = a->rope_sin, n.max_pos = a->rope_max_pos;
+    n.positions = a->positions, n.slots = a->slots;
+    if (a->cache) n.cache = pages_of(*a->cache);
+    n.rows = (int32_t)a->rows, n.group = a->n_heads / a->n_kv_heads, n.kv_heads = a->n_kv_heads;
+    n.eps = a->eps;
+    n.vec = moves4(a->q, a->q_stride, dt) && moves4(a->k, a->k_stride, dt) && (!a->cache || moves4(a->v, a->v_stride, dt)) &&
+            moves4(a->q_out, a->q_out_stride, dt) && moves4(a->k_out, a->k_out_stride, dt) && kv4_aligned(a->rope_cos, 16) &&
+            kv4_aligned(a->rope_sin, 16) && kv4_aligned(a->q_norm, 8) && kv4_aligned(a->k_norm, 8);
+    DeviceGuard guard(c->device);
+    return kv4_done(c, enqueue_qk_norm_rope(n, dt, D, a->cache != nullptr, (hipStream_t)stream));
+}
+
+extern "C" int qtts_kv4_gather(qtts_ctx *c, const qtts_kv4 *cache, const int64_t *slots, int64_t n, int32_t dtype, void *K,
+                               void *V, void *stream, int flags)
+{
+    if (!c && !(flags & QTTS_CHECK_ONLY)) return QTTS_ERR_INVALID;
+    RCHK(check_dtype(c, dtype));
+    RCHK(check_kv4(c, cache));
+    if (n < 0 || (n && !slots) || !kv4_aligned(slots, 8)) return fail(c, QTTS_ERR_INVALID, "slots null or not aligned, or a negative count");
+    if (n > (1 << 27) / (int64_t)cache->n_kv_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 slots x heads a call");
+    const int64_t bytes = n * cache->n_kv_heads * cache->head_dim * kv4_size(dtype);
+    if (!kv4_aligned(K, (size_t)(4 * kv4_size(dtype))) || !kv4_aligned(V, (size_t)(4 * kv4_size(dtype))))
+        return fail(c, QTTS_ERR_INVALID, "K and V must be aligned to four elements");
+    const Rows k = flat(K, bytes), v = flat(V, bytes), s = flat(slots, 8 * n), pages = rows_of(*cache);
+    if (rows_clash(k, v) || rows_clash(k, s) || rows_clash(v, s) || rows_clash(k, pages) || rows_clash(v, pages))
+        return fail(c, QTTS_ERR_INVALID, "an output overlaps another array");
+    if ((flags & QTTS_CHECK_ONLY) || n == 0 || (!K && !V)) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    return kv4_done(c, enqueue_kv4_gather(pages_of(*cache), cache->head_dim, slots, (int)n, dtype, K, V, (hipStream_t)stream));
+}
+
+// Everything but the workspace.
+static int check_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a)
+{
+    RCHK(check_dtype(c, a->dtype));
+    RCHK(check_kv4(c, a->cache));
+    const int D = a->cache->head_dim;
+    if (a->rows < 0 || a->n_seqs < 0 || a->n_heads < 1 || a->n_heads % a->cache->n_kv_heads)
+        return fail(c, QTTS_ERR_INVALID, "%lld rows, %d sequences, %d / %d heads", (long long)a->rows, a->n_seqs, a->n_heads,
+                    a->cache->n_kv_heads);
+    if (a->rows > (1 << 27) / (int64_t)a->n_heads || a->n_seqs > (1 << 22))
+        return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 rows x heads and 2^22 sequences a call");
+    RCHK(check_rows(c, "q", a->q, a->rows, a->n_heads, D, a->q_stride, a->dtype));
+    RCHK(check_rows(c, "out", a->out, a->rows, a->n_heads, D, a->out_stride, a->dtype));
+    if (a->max_pages < 1 || a->table_stride < a->max_pages || a->max_pages > INT32_MAX / KV4_PAGE - 2 || a->table_stride > INT32_MAX)
+        return fail(c, QTTS_ERR_INVALID, "table of %d columns, row stride %lld", a->max_pages, (long long)a->table_stride);
+    if (a->n_seqs && (!a->row_start || !a->lengths || !a->table)) return fail(c, QTTS_ERR_INVALID, "null array");
+    if (!kv4_aligned(a->row_start, 4) || !kv4_aligned(a->lengths, 4) || !kv4_aligned(a->table, 4))
+        return fail(c, QTTS_ERR_INVALID, "array not aligned to its element type");
+    if (!std::isfinite(a->scale) || a->scale == 0.0f) return fail(c, QTTS_ERR_INVALID, "scale %g", a->scale);
+    if (a->window < 0 || a->max_len < 0) return fail(c, QTTS_ERR_INVALID, "negative window or length");
+    const int64_t sz = kv4_size(a->dtype);
+    const Rows q = {a->q, a->rows, a->q_stride * sz, a->n_heads * D * sz}, o = {a->out, a->rows, a->out_stride * sz, a->n_heads * D * sz},
+               t = {a->table, a->n_seqs, 4 * a->table_stride, 4LL * a->max_pages};
+    if ((!(a->out == a->q && a->out_stride == a->q_stride) && rows_clash(q, o)) || rows_clash(o, rows_of(*a->cache)) ||
+        rows_clash(o, t) || rows_clash(o, flat(a->row_start, 4LL * (a->n_seqs + 1))) || rows_clash(o, flat(a->lengths, 4LL * a->n_seqs)))
+        return fail(c, QTTS_ERR_INVALID, "out overlaps another array");
+    return QTTS_OK;
+}
+
+static int attention_splits(const qtts_kv4_attention_args *a)
+{
+    return kv4_attn_splits(a->rows, a->n_seqs, a->n_heads / a->cache->n_kv_heads, a->cache->n_kv_heads, a->max_len, a->window);
+}
+
+// Floats of the partial results: maxima and sums, then rows.
+static int64_t attention_parts(const qtts_kv4_attention_args *a)
+{
+    return kv4_first_tile(a->rows, a->n_heads / a->cache->n_kv_heads, a->n_seqs, KV4_W) * a->cache->n_kv_heads * attention_splits(a);
+}
+
+extern "C" int qtts_kv4_attention_workspace(const qtts_kv4_attention_args *a, int64_t *bytes)
+{
+    if (!a || !bytes) return QTTS_ERR_INVALID;
+    RCHK(check_kv4_attention(nullptr, a));
+    *bytes = a->rows && a->n_seqs && attention_splits(a) > 1 ? attention_parts(a) * (32 + KV4_W * a->cache->head_dim) * 4 : 0;
+    return QTTS_OK;
+}
+
+extern "C" int qtts_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a, void *stream, int flags)
+{
+    if (!a || (!c && !(flags & QTTS_CHECK_ONLY))) return QTTS_ERR_INVALID;
+    RCHK(check_kv4_attention(c, a));
+    int64_t need = 0;
+    RCHK(qtts_kv4_attention_workspace(a, &need));
+    if (need > a->workspace_bytes || (need && !a->workspace) || (need && !kv4_aligned(a->workspace, 16)))
+        return fail(c, QTTS_ERR_CAPACITY, "workspace of %lld bytes, 16-byte aligned, needed; %lld given", (long long)need,
+                    (long long)a->workspace_bytes);
+    const int64_t sz = kv4_size(a->dtype), D = a->cache->head_dim, width = a->n_heads * D * sz;
+    const Rows w = need ? flat(a->workspace, need) : Rows{};
+    if (rows_clash(w, {a->q, a->rows, a->q_stride * sz, width}) || rows_clash(w, {a->out, a->rows, a->out_stride * sz, width}) ||
+        rows_clash(w, rows_of(*a->cache)) || rows_clash(w, {a->table, a->n_seqs, 4 * a->table_stride, 4LL * a->max_pages}) ||
+        rows_clash(w, flat(a->row_start, 4LL * (a->n_seqs + 1))) || rows_clash(w, flat(a->lengths, 4LL * a->n_seqs)))
+        return fail(c, QTTS_ERR_INVALID, "the workspace overlaps another array");
+    if ((flags & QTTS_CHECK_ONLY) || a->rows == 0 || a->n_seqs == 0) return QTTS_OK;
+    Kv4Attn k{};
+    k.q = a->q, k.out = a->out, k.q_stride = a->q_stride, k.out_stride = a->out_stride;
+    k.cache = pages_of(*a->cache);
+    k.row_start = a->row_start, k.lengths = a->lengths, k.table = a->table, k.table_stride = a->table_stride;
+    k.part = (float *)a->workspace;
+    k.rows = (int32_t)a->rows, k.n_seqs = a->n_seqs, k.max_pages = a->max_pages, k.group = a->n_heads / a->cache->n_kv_heads;
+    k.window = a->window, k.splits = attention_splits(a), k.scale = a->scale;
+    k.part_rows = 32 * attention_parts(a);
+    k.vec = moves4(a->q, a->q_stride, a->dtype) && moves4(a->out, a->out_stride, a->dtype);
+    DeviceGuard guard(c->device);
+    return kv4_done(c, enqueue_kv4_attn(k, a->dtype, (int)D, (hipStream_t)stream));
 }
 
 // ---------------------------------------------------------------------------

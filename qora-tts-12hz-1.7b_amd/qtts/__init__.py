@@ -12,6 +12,9 @@ The functions mirror the reference crate's forward-call surface:
     sample_token                      generate_new.rs:771
     frame loop                        generate_new.rs:606-675
 
+and, without a counterpart there, the operators between the linear maps of a
+program that serves many sequences over a 4-bit cache (kv4.py).
+
 Every call goes through the C ABI; there is no CPU fallback.  A missing or
 unloadable library raises QttsError.
 """
@@ -21,7 +24,8 @@ from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int32, 
 
 import numpy as np
 
-from . import hostdesc
+from . import hostdesc, kv4
+from .kv4 import Kv4Cache, Kv4Step, kv4_page_bytes
 from .hostdesc import DecoderHost, PredictorHost, Q4Host, SampleParams, TalkerHost, decoder_host, ptr, sample_params
 
 
@@ -43,6 +47,7 @@ TILE_SHAPES = [(256, 8, 8), (128, 8, 8), (64, 1, 8), (128, 1, 8), (256, 1, 8), (
 
 OK, ERR_INVALID, ERR_HIP, ERR_OOM, ERR_CAPACITY, ERR_STATE, ERR_IO, ERR_NAN, ERR_UNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7, -8
 DEVICE_PTRS = 1
+CHECK_ONLY = 8
 PATH_ROWWISE, PATH_MFMA = 2, 4
 _PATH_FLAGS = {None: 0, "rowwise": PATH_ROWWISE, "mfma": PATH_MFMA}
 
@@ -88,6 +93,12 @@ SIGNATURES = {
     "qtts_build_trailing_text": ([c_void_p, c_void_p, c_int64, c_void_p, c_int], c_int),
     "qtts_prefill_custom_voice": ([c_void_p, c_void_p, c_int64, c_uint32, c_uint32, c_void_p, c_int64, c_void_p,
                                    c_int64, c_void_p, c_void_p, POINTER(c_int64), c_int], c_int),
+    "qtts_kv4_tables": ([c_void_p, POINTER(hostdesc.Kv4TablesArgs), c_void_p, c_int], c_int),
+    "qtts_qk_norm_rope": ([c_void_p, POINTER(hostdesc.QkNormRopeArgs), c_void_p, c_int], c_int),
+    "qtts_kv4_gather": ([c_void_p, POINTER(hostdesc.Kv4), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
+                         c_int], c_int),
+    "qtts_kv4_attention_workspace": ([POINTER(hostdesc.Kv4AttentionArgs), POINTER(c_int64)], c_int),
+    "qtts_kv4_attention": ([c_void_p, POINTER(hostdesc.Kv4AttentionArgs), c_void_p, c_int], c_int),
     "qtts_decoder_upload": ([c_void_p, POINTER(DecoderHost)], c_int),
     "qtts_decoder_dims": ([c_void_p, POINTER(c_int32), POINTER(c_int32), POINTER(c_int64)], c_int),
     "qtts_decode_to_audio": ([c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, POINTER(c_int64),
@@ -178,6 +189,7 @@ class Context:
         if rc != OK:
             raise QttsError(rc, "qtts_ctx_create failed (no HIP device?)")
         self.h = h
+        self.device = device
         self._keep = []
         self.dec_codebooks = 16
 
@@ -397,6 +409,13 @@ class Context:
             0 if v is None else v.size, ptr(icl) if icl is not None else None, 0 if icl is None else icl.shape[0],
             ptr(hid), ptr(lg), byref(pos), _PATH_FLAGS[path]))
         return hid, lg, pos.value
+
+    # ---- many sequences over a 4-bit cache ------------------------------------
+    # on torch tensors of the context's device (kv4.py)
+    kv4_tables = kv4.tables
+    qk_norm_rope = kv4.qk_norm_rope
+    kv4_gather = kv4.gather
+    kv4_attention = kv4.attention
 
     # ---- speech decoder -----------------------------------------------------
     def upload_decoder(self, decoder):

@@ -225,3 +225,36 @@ def decoder_host(d):
         ptr(d.final_snake_alpha), ptr(d.final_snake_beta), conv1d_host(d.output_conv),
         ptr(d.rope_cos), ptr(d.rope_sin), d.rope_cos.shape[0])
     return h, (rest, layers, ups, res_arrays, vb)
+
+
+class Kv4(ctypes.Structure):
+    """qtts_kv4: one layer's pages of a 4-bit cache."""
+    _fields_ = [("base", c_void_p), ("n_pages", c_int64), ("page_stride", c_int64), ("n_kv_heads", c_int32),
+                ("head_dim", c_int32)]
+
+
+class Kv4TablesArgs(ctypes.Structure):
+    """qtts_kv4_tables_args."""
+    _fields_ = [("n_seqs", c_int32), ("max_pages", c_int32), ("cached", c_void_p), ("fresh", c_void_p),
+                ("free_pages", c_void_p), ("n_free", c_int64), ("table", c_void_p), ("table_stride", c_int64),
+                ("row_start", c_void_p), ("lengths", c_void_p), ("positions", c_void_p), ("slots", c_void_p),
+                ("n_rows", c_int64), ("status", c_void_p)]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    """qtts_qk_norm_rope_args."""
+    _fields_ = [("dtype", c_int32), ("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32),
+                ("rows", c_int64), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_stride", c_int64),
+                ("k_stride", c_int64), ("v_stride", c_int64), ("q_out", c_void_p), ("k_out", c_void_p),
+                ("q_out_stride", c_int64), ("k_out_stride", c_int64), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("eps", c_float), ("reserved", c_int32), ("rope_cos", c_void_p), ("rope_sin", c_void_p),
+                ("rope_max_pos", c_int64), ("positions", c_void_p), ("cache", ctypes.POINTER(Kv4)), ("slots", c_void_p)]
+
+
+class Kv4AttentionArgs(ctypes.Structure):
+    """qtts_kv4_attention_args."""
+    _fields_ = [("dtype", c_int32), ("n_heads", c_int32), ("rows", c_int64), ("q", c_void_p), ("out", c_void_p),
+                ("q_stride", c_int64), ("out_stride", c_int64), ("cache", ctypes.POINTER(Kv4)), ("n_seqs", c_int32),
+                ("max_pages", c_int32), ("row_start", c_void_p), ("lengths", c_void_p), ("table", c_void_p),
+                ("table_stride", c_int64), ("max_len", c_int64), ("scale", c_float), ("window", c_int32),
+                ("workspace", c_void_p), ("workspace_bytes", c_int64)]
