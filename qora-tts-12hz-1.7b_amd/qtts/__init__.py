@@ -93,12 +93,11 @@ SIGNATURES = {
     "qtts_build_trailing_text": ([c_void_p, c_void_p, c_int64, c_void_p, c_int], c_int),
     "qtts_prefill_custom_voice": ([c_void_p, c_void_p, c_int64, c_uint32, c_uint32, c_void_p, c_int64, c_void_p,
                                    c_int64, c_void_p, c_void_p, POINTER(c_int64), c_int], c_int),
-    "qtts_kv4_tables": ([c_void_p, POINTER(hostdesc.Kv4TablesArgs), c_void_p, c_int], c_int),
-    "qtts_qk_norm_rope": ([c_void_p, POINTER(hostdesc.QkNormRopeArgs), c_void_p, c_int], c_int),
-    "qtts_kv4_gather": ([c_void_p, POINTER(hostdesc.Kv4), c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
-                         c_int], c_int),
-    "qtts_kv4_attention_workspace": ([POINTER(hostdesc.Kv4AttentionArgs), POINTER(c_int64)], c_int),
-    "qtts_kv4_attention": ([c_void_p, POINTER(hostdesc.Kv4AttentionArgs), c_void_p, c_int], c_int),
+    "qtts_kv4_tables": ([c_void_p, c_void_p, c_void_p, c_int], c_int),
+    "qtts_qk_norm_rope": ([c_void_p, c_void_p, c_void_p, c_int], c_int),
+    "qtts_kv4_gather": ([c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_int], c_int),
+    "qtts_kv4_attention_workspace": ([c_void_p, c_void_p], c_int),
+    "qtts_kv4_attention": ([c_void_p, c_void_p, c_void_p, c_int], c_int),
     "qtts_decoder_upload": ([c_void_p, POINTER(DecoderHost)], c_int),
     "qtts_decoder_dims": ([c_void_p, POINTER(c_int32), POINTER(c_int32), POINTER(c_int64)], c_int),
     "qtts_decode_to_audio": ([c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, POINTER(c_int64),

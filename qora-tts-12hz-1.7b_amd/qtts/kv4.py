@@ -5,16 +5,35 @@ qtts_kv4_gather, qtts_kv4_attention of include/qtts.h).
 Each call only enqueues kernels, on torch's current stream of the context's
 device, and may be captured into a graph.  Results and workspaces come from
 torch's allocator unless `out` arguments are given.
+
+A decode step makes these calls in every layer, so a call's way to its launch
+counts as its kernel does: arguments are packed into the C structs' bytes
+(their ctypes mirrors are in hostdesc.py), and what a tensor is gets checked by
+identity and plain numbers.
 """
 import ctypes
 import math
+import struct
 import sys
 
-from .hostdesc import Kv4, Kv4AttentionArgs, Kv4TablesArgs, QkNormRopeArgs
+from .hostdesc import Kv4
 
 PAGE = 64
-_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-_by_dtype = {}               # torch dtype -> QTTS_F32 / F16 / BF16
+_TABLES = struct.Struct("@iiPPPqPqPPPPqP")                 # qtts_kv4_tables_args
+_POST = struct.Struct("@iiiiqPPPqqqPPqqPPfiPPqPPP")        # qtts_qk_norm_rope_args
+_ATTENTION = struct.Struct("@iiqPPqqPiiPPPqqfiPq")         # qtts_kv4_attention_args
+
+_torch = None                # the module, once a tensor has come
+_codes = {}                  # torch dtype -> QTTS_F32 / F16 / BF16
+_stream = None               # device -> torch's current stream
+
+
+def _load():
+    global _torch, _stream
+    t = sys.modules["torch"]     # whoever passes its tensors has imported it
+    _codes.update({t.float32: 0, t.float16: 1, t.bfloat16: 2})
+    _stream = t._C._cuda_getCurrentRawStream
+    _torch = t
 
 
 def kv4_page_bytes(n_kv_heads, head_dim):
@@ -22,52 +41,49 @@ def kv4_page_bytes(n_kv_heads, head_dim):
     return n_kv_heads * 72 * head_dim
 
 
-def _dtype(t):
-    code = _by_dtype.get(t)
+def _code(name, t):
+    code = _codes.get(t.dtype)
     if code is None:
-        code = _DTYPES.get(str(t))
-        if code is None:
-            raise TypeError(f"rows are float32, float16 or bfloat16, not {t}")
-        _by_dtype[t] = code
+        raise TypeError(f"{name}: float32, float16 or bfloat16 expected, got {t.dtype}")
     return code
 
 
-def _torch():
-    return sys.modules["torch"]  # whoever passes its tensors has imported it
+def _elsewhere(name, t, device):
+    return ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
 
 
-def _stream(ctx):
-    return _torch()._C._cuda_getCurrentRawStream(ctx.device)
-
-
-def _on(ctx, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
-            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
-
-
-def _vector(name, t, n, dtype):
-    """A contiguous vector of n (None: any number) whole numbers of that type."""
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or str(t.dtype) != dtype or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous {dtype} [{'n' if n is None else n}] expected, got {t.dtype} {list(t.shape)}")
+def _vector(name, t, n, dtype, device):
+    """The address of a contiguous vector of n values of that type."""
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype} [{n}] expected, got {t.dtype} {list(t.shape)}")
+    if t.get_device() != device:
+        raise _elsewhere(name, t, device)
     return t.data_ptr()
 
 
-def _rows(name, t, heads=None, dim=None, dtype=None):
+def _rows(name, t, rows, heads, dim, dtype, device):
     """[rows][heads][dim] with whole heads next to each other: the row stride."""
-    if t.dim() != 3 or (heads is not None and tuple(t.shape[1:]) != (heads, dim)):
-        raise ValueError(f"{name}: [rows][{heads or 'heads'}][{dim or 'dim'}] expected, got {list(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
+    shape = t.shape
+    if t.dim() != 3 or shape[0] != rows or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name}: [{rows}][{heads}][{dim}] expected, got {list(shape)}")
+    if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, not {dtype}")
-    if t.shape[0] and ((t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+    if t.get_device() != device:
+        raise _elsewhere(name, t, device)
+    if rows == 0:
+        return heads * dim
+    s = t.stride()
+    if s[2] != 1 or (heads > 1 and s[1] != dim):
         raise ValueError(f"{name}: the heads of a row must lie next to each other")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return s[0] if rows > 1 else heads * dim
 
 
-def _table(t, n):
+def _table(t, n, device):
     """[n][max_pages] int32 with the entries of a row next to each other: the row stride."""
-    if t.dim() != 2 or t.shape[0] != n or str(t.dtype) != "torch.int32" or (n and t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dim() != 2 or t.shape[0] != n or t.dtype is not _torch.int32 or (n and t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"table: int32 [{n}][max_pages] expected, got {t.dtype} {list(t.shape)}")
+    if t.get_device() != device:
+        raise _elsewhere("table", t, device)
     return t.stride(0) if n > 1 else t.shape[1]
 
 
@@ -76,17 +92,28 @@ class Kv4Cache:
     (trailing dimensions may be split; pages may lie further apart)."""
 
     def __init__(self, pages, n_kv_heads, head_dim):
-        size = kv4_page_bytes(n_kv_heads, head_dim)
-        if str(pages.dtype) != "torch.uint8" or pages.dim() < 2 or pages[0].numel() != size or not pages[0].is_contiguous():
-            raise ValueError(f"pages: uint8 [n][{size}] expected, got {pages.dtype} {list(pages.shape)}")
+        if _torch is None:
+            _load()
+        size, inner = n_kv_heads * 72 * head_dim, 1
+        shape, strides = pages.shape, pages.stride()
+        n = shape[0] if shape else 0
+        for d in range(len(shape) - 1, 0, -1):
+            if shape[d] > 1 and strides[d] != inner:
+                inner = -1
+                break
+            inner *= shape[d]
+        if pages.dtype is not _torch.uint8 or len(shape) < 2 or inner != size:
+            raise ValueError(f"pages: uint8 [n][{size}] expected, got {pages.dtype} {list(shape)}")
         self.pages, self.n_kv_heads, self.head_dim = pages, n_kv_heads, head_dim
-        stride = pages.stride(0) if pages.shape[0] > 1 else size
-        self.desc = Kv4(pages.data_ptr(), pages.shape[0], stride, n_kv_heads, head_dim)
+        self.device = pages.get_device()
+        self.desc = Kv4(pages.data_ptr(), n, strides[0] if n > 1 else size, n_kv_heads, head_dim)
+        self.address = ctypes.addressof(self.desc)
 
 
 class Kv4Step:
     """What one step's rows are: row_start, lengths, positions and slots for the
     operators, and status, which check() reads (it waits for the device)."""
+    __slots__ = ("row_start", "lengths", "positions", "slots", "status")
 
     def __init__(self, row_start, lengths, positions, slots, status):
         self.row_start, self.lengths, self.positions, self.slots, self.status = row_start, lengths, positions, slots, status
@@ -105,21 +132,22 @@ def tables(self, cached, fresh, free_pages, table, rows, out=None):
     [n_seqs] int32, free_pages [n] int32, table [n_seqs][max_pages] int32
     (written in place), `rows` the room for rows.  Returns a Kv4Step (out: one
     to write into)."""
-    n = cached.shape[0]
-    _on(self, cached=cached, fresh=fresh, free_pages=free_pages, table=table)
+    if _torch is None:
+        _load()
+    device, i32 = self.device, _torch.int32
+    n, free = cached.shape[0], free_pages.shape[0]
     if out is None:
-        i32 = cached.dtype
-        out = Kv4Step(cached.new_empty(n + 1), cached.new_empty(n), cached.new_empty(rows),
-                      cached.new_empty(rows, dtype=_torch().int64), cached.new_empty(2, dtype=i32))
-    else:
-        _on(self, row_start=out.row_start, lengths=out.lengths, positions=out.positions, slots=out.slots, status=out.status)
-    stride = _table(table, n)
-    a = Kv4TablesArgs(n, table.shape[1], _vector("cached", cached, n, "torch.int32"), _vector("fresh", fresh, n, "torch.int32"),
-                      _vector("free_pages", free_pages, None, "torch.int32"), free_pages.shape[0], table.data_ptr(), stride,
-                      _vector("row_start", out.row_start, n + 1, "torch.int32"), _vector("lengths", out.lengths, n, "torch.int32"),
-                      _vector("positions", out.positions, rows, "torch.int32"), _vector("slots", out.slots, rows, "torch.int64"),
-                      rows, _vector("status", out.status, 2, "torch.int32"))
-    self._check(self.lib.qtts_kv4_tables(self.h, ctypes.byref(a), _stream(self), 0))
+        # one allocation for what is held in 32 bits
+        row_start, lengths, positions, status = cached.new_empty(2 * n + rows + 3).split_with_sizes([n + 1, n, rows, 2])
+        out = Kv4Step(row_start, lengths, positions, cached.new_empty(rows, dtype=_torch.int64), status)
+    a = _TABLES.pack(n, table.shape[1], _vector("cached", cached, n, i32, device), _vector("fresh", fresh, n, i32, device),
+                     _vector("free_pages", free_pages, free, i32, device), free, table.data_ptr(), _table(table, n, device),
+                     _vector("row_start", out.row_start, n + 1, i32, device), _vector("lengths", out.lengths, n, i32, device),
+                     _vector("positions", out.positions, rows, i32, device),
+                     _vector("slots", out.slots, rows, _torch.int64, device), rows, _vector("status", out.status, 2, i32, device))
+    rc = self.lib.qtts_kv4_tables(self.h, a, _stream(device), 0)
+    if rc:
+        self._check(rc)
     return out
 
 
@@ -131,57 +159,64 @@ def qk_norm_rope(self, q, k, positions=None, cos=None, sin=None, q_norm=None, k_
     positions [rows] int32, q_norm and k_norm [dim] f16; None leaves that part
     out.  Returns (q_out, k_out); with a cache k is only written out where k_out
     is given."""
-    _on(self, q=q, k=k, v=v, positions=positions, cos=cos, sin=sin, q_norm=q_norm, k_norm=k_norm, slots=slots, q_out=q_out, k_out=k_out)
+    if _torch is None:
+        _load()
+    device, dtype = self.device, q.dtype
     rows, heads, dim = q.shape
-    dtype = q.dtype
-    code = _dtype(dtype)
-    q_stride = _rows("q", q)
-    k_stride = _rows("k", k, k.shape[1], dim, dtype)
-    if k.shape[0] != rows:
-        raise ValueError(f"k has {k.shape[0]} rows, q {rows}")
+    kv_heads = k.shape[1]
+    code = _code("q", q)
+    q_stride = _rows("q", q, rows, heads, dim, dtype, device)
+    k_stride = _rows("k", k, rows, kv_heads, dim, dtype, device)
     if q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out, qo_stride = _torch.empty_like(q, memory_format=_torch.contiguous_format), heads * dim
+    else:
+        qo_stride = _rows("q_out", q_out, rows, heads, dim, dtype, device)
     if k_out is None and cache is None:
-        k_out = k.new_empty(k.shape)
-    a = QkNormRopeArgs(code, heads, k.shape[1], dim, rows, q.data_ptr(), k.data_ptr(), None, q_stride, k_stride, 0,
-                       q_out.data_ptr(), None, _rows("q_out", q_out, heads, dim, dtype))
-    if q_out.shape[0] != rows or (k_out is not None and k_out.shape[0] != rows):
-        raise ValueError("outputs must have as many rows as q")
-    if k_out is not None:
-        a.k_out, a.k_out_stride = k_out.data_ptr(), _rows("k_out", k_out, k.shape[1], dim, dtype)
-    if q_norm is not None:
-        a.q_norm = _vector("q_norm", q_norm, dim, "torch.float16")
-    if k_norm is not None:
-        a.k_norm = _vector("k_norm", k_norm, dim, "torch.float16")
-    a.eps = eps
+        k_out = _torch.empty_like(k, memory_format=_torch.contiguous_format)
+    ko, ko_stride = (0, 0) if k_out is None else (k_out.data_ptr(), _rows("k_out", k_out, rows, kv_heads, dim, dtype, device))
+    at = cos_at = sin_at = most = vp = v_stride = desc = slots_at = 0
     if positions is not None:
-        if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != dim // 2 or \
-                str(cos.dtype) != "torch.float32" or cos.dtype != sin.dtype or not cos.is_contiguous() or not sin.is_contiguous():
-            raise ValueError(f"cos and sin: contiguous float32 [max_pos][{dim // 2}] expected")
-        a.rope_cos, a.rope_sin, a.rope_max_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        a.positions = _vector("positions", positions, rows, "torch.int32")
+        if cos is None or sin is None:
+            raise ValueError("positions need cos and sin")
+        most = cos.shape[0]
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype is not _torch.float32 or t.dim() != 2 or t.shape[0] != most or t.shape[1] != dim // 2 or not t.is_contiguous():
+                raise ValueError(f"{name}: contiguous float32 [{most}][{dim // 2}] expected, got {t.dtype} {list(t.shape)}")
+            if t.get_device() != device:
+                raise _elsewhere(name, t, device)
+        at, cos_at, sin_at = _vector("positions", positions, rows, _torch.int32, device), cos.data_ptr(), sin.data_ptr()
     if cache is not None:
         if v is None or slots is None:
             raise ValueError("a cache needs v and slots")
-        _on(self, pages=cache.pages)
-        a.v, a.v_stride = v.data_ptr(), _rows("v", v, k.shape[1], dim, dtype)
-        if v.shape[0] != rows:
-            raise ValueError(f"v has {v.shape[0]} rows, q {rows}")
-        a.cache = ctypes.pointer(cache.desc)
-        a.slots = _vector("slots", slots, rows, "torch.int64")
-    self._check(self.lib.qtts_qk_norm_rope(self.h, ctypes.byref(a), _stream(self), 0))
+        if cache.device != device:
+            raise _elsewhere("the cache", cache.pages, device)
+        vp, v_stride, desc = v.data_ptr(), _rows("v", v, rows, kv_heads, dim, dtype, device), cache.address
+        slots_at = _vector("slots", slots, rows, _torch.int64, device)
+    a = _POST.pack(code, heads, kv_heads, dim, rows, q.data_ptr(), k.data_ptr(), vp, q_stride, k_stride, v_stride,
+                   q_out.data_ptr(), ko, qo_stride, ko_stride,
+                   0 if q_norm is None else _vector("q_norm", q_norm, dim, _torch.float16, device),
+                   0 if k_norm is None else _vector("k_norm", k_norm, dim, _torch.float16, device),
+                   eps, 0, cos_at, sin_at, most, at, desc, slots_at)
+    rc = self.lib.qtts_qk_norm_rope(self.h, a, _stream(device), 0)
+    if rc:
+        self._check(rc)
     return q_out, k_out
 
 
 def gather(self, cache, slots, dtype):
     """The keys and values held at `slots` [n] int64 (qtts_kv4_gather): two
     tensors [n][kv_heads][dim] of `dtype`, zero for a slot outside the pages."""
-    _on(self, slots=slots, pages=cache.pages)
+    if _torch is None:
+        _load()
+    device = self.device
+    if cache.device != device:
+        raise _elsewhere("the cache", cache.pages, device)
     n = slots.shape[0]
-    shape = (n, cache.n_kv_heads, cache.head_dim)
-    K, V = slots.new_empty(shape, dtype=dtype), slots.new_empty(shape, dtype=dtype)
-    self._check(self.lib.qtts_kv4_gather(self.h, ctypes.byref(cache.desc), _vector("slots", slots, None, "torch.int64"), n,
-                                         _dtype(dtype), K.data_ptr(), V.data_ptr(), _stream(self), 0))
+    at = _vector("slots", slots, n, _torch.int64, device)
+    K, V = slots.new_empty((2, n, cache.n_kv_heads, cache.head_dim), dtype=dtype).unbind()
+    rc = self.lib.qtts_kv4_gather(self.h, cache.address, at, n, _code("values", K), K.data_ptr(), V.data_ptr(), _stream(device), 0)
+    if rc:
+        self._check(rc)
     return K, V
 
 
@@ -191,25 +226,32 @@ def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, m
     lengths [n_seqs] int32.  scale None: 1 / sqrt(dim).  max_len, an upper
     bound of the lengths, helps to split the work.  Rows outside all sequences
     are left as they are in `out`."""
-    _on(self, q=q, table=table, row_start=row_start, lengths=lengths, out=out, pages=cache.pages)
-    rows, heads, dim = q.shape
-    n = lengths.shape[0]
-    if dim != cache.head_dim:
-        raise ValueError(f"q has heads of {dim}, the cache of {cache.head_dim}")
+    if _torch is None:
+        _load()
+    device, dtype, i32 = self.device, q.dtype, _torch.int32
+    dim, n = cache.head_dim, lengths.shape[0]
+    if cache.device != device:
+        raise _elsewhere("the cache", cache.pages, device)
+    if q.dim() != 3:
+        raise ValueError(f"q: [rows][heads][{dim}] expected, got {list(q.shape)}")
+    rows, heads = q.shape[0], q.shape[1]
+    code, q_stride = _code("q", q), _rows("q", q, rows, heads, dim, dtype, device)
     if out is None:
-        out = q.new_empty(q.shape)
-    elif out.shape[0] != rows:
-        raise ValueError(f"out has {out.shape[0]} rows, q {rows}")
-    a = Kv4AttentionArgs(_dtype(q.dtype), heads, rows, q.data_ptr(), out.data_ptr(), _rows("q", q),
-                         _rows("out", out, heads, dim, q.dtype), ctypes.pointer(cache.desc), n, table.shape[1],
-                         _vector("row_start", row_start, n + 1, "torch.int32"), _vector("lengths", lengths, n, "torch.int32"),
-                         table.data_ptr(), _table(table, n),
-                         PAGE * table.shape[1] if max_len is None else max_len, 1 / math.sqrt(dim) if scale is None else scale,
-                         window, None, 0)
+        out, out_stride = _torch.empty_like(q, memory_format=_torch.contiguous_format), heads * dim
+    else:
+        out_stride = _rows("out", out, rows, heads, dim, dtype, device)
+    columns = table.shape[1] if table.dim() == 2 else 0
+    head = (code, heads, rows, q.data_ptr(), out.data_ptr(), q_stride, out_stride, cache.address, n, columns,
+            _vector("row_start", row_start, n + 1, i32, device), _vector("lengths", lengths, n, i32, device), table.data_ptr(),
+            _table(table, n, device), PAGE * columns if max_len is None else max_len, 1 / math.sqrt(dim) if scale is None else scale,
+            window)
+    a = _ATTENTION.pack(*head, 0, 0)
     need = ctypes.c_int64()
-    rc = self.lib.qtts_kv4_attention_workspace(ctypes.byref(a), ctypes.byref(need))
-    if rc == 0 and need.value:
-        workspace = q.new_empty(need.value, dtype=_torch().uint8)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need.value
-    self._check(self.lib.qtts_kv4_attention(self.h, ctypes.byref(a), _stream(self), 0))
+    self.lib.qtts_kv4_attention_workspace(a, ctypes.byref(need))     # what it refuses the call itself names
+    if need.value:
+        workspace = q.new_empty(need.value, dtype=_torch.uint8)
+        a = _ATTENTION.pack(*head, workspace.data_ptr(), need.value)
+    rc = self.lib.qtts_kv4_attention(self.h, a, _stream(device), 0)
+    if rc:
+        self._check(rc)
     return out

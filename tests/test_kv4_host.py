@@ -26,6 +26,14 @@ def test_layouts():
     assert ctypes.sizeof(QkNormRopeArgs) == 176 and QkNormRopeArgs.rope_max_pos.offset == 144 and QkNormRopeArgs.slots.offset == 168
     assert Kv4AttentionArgs.window.offset == 108 and ctypes.sizeof(Kv4AttentionArgs) == 128
     assert qtts.kv4_page_bytes(8, 128) == 73728
+    from qtts import kv4
+    for packed, mirror in ((kv4._TABLES, Kv4TablesArgs), (kv4._POST, QkNormRopeArgs), (kv4._ATTENTION, Kv4AttentionArgs)):
+        assert packed.size == ctypes.sizeof(mirror)
+        fields = [f for f, _ in mirror._fields_]
+        got = mirror.from_buffer_copy(packed.pack(*range(1, len(fields) + 1)))
+        values = [getattr(got, f) for f in fields]
+        values = [ctypes.cast(v, ctypes.c_void_p).value if isinstance(v, ctypes._Pointer) else v for v in values]
+        assert values == list(range(1, len(fields) + 1))
 
 
 def cache(**kw):
