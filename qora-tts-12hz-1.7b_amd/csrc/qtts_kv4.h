@@ -61,7 +61,7 @@ struct Kv4Attn {
     float *part;                     // splits > 1: [tile][kv head][split] {16 maxima, 16 sums}, then the rows
     int64_t part_rows;               // floats before the rows
     int32_t rows, n_seqs, max_pages, group;
-    int32_t window, splits;
+    int32_t window, chunk, splits;   // pages of a workgroup, most workgroups of a tile
     float scale;
     int32_t vec;
 };
@@ -77,7 +77,7 @@ __host__ __device__ constexpr int64_t kv4_first_tile(int64_t row, int group, int
 hipError_t enqueue_kv4_tables(const Kv4Tables &a, hipStream_t s);
 hipError_t enqueue_qk_norm_rope(const QkNormRope &a, int dtype, int D, bool store, hipStream_t s);
 hipError_t enqueue_kv4_gather(const Kv4Pages &c, int D, const int64_t *slots, int n, int dtype, void *K, void *V, hipStream_t s);
-int kv4_attn_splits(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window);
+void kv4_attn_split(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window, int *chunk, int *splits);
 hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, hipStream_t s);
 
 }  // namespace qtts

@@ -480,20 +480,29 @@ __device__ __forceinline__ float add_xor16(float v)
 __device__ __forceinline__ h16x2 as_h2(uint32_t u) { return __builtin_bit_cast(h16x2, u); }
 __device__ __forceinline__ uint32_t as_u(h16x2 h) { return __builtin_bit_cast(uint32_t, h); }
 
+// Masks and exponents of unpack8 where one v_and_or_b32 can take both: a
+// VALU instruction reads one scalar register and no literal beside it, so the
+// masks are kept in scalar registers and the exponent in a vector register
+// (as constants they cost an and and an or: 128 instructions of 866 a page).
+struct Unpack {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, one = 0x64006400u;
+    __device__ __forceinline__ Unpack() { asm volatile("" : "+s"(low), "+s"(high), "+v"(one)); }
+};
+
 // Eight codes (four bits at 0, 4, 8 and 12 of each half of w) times scales, as
 // f16 pairs: out[n] = (code n of the low half, code n of the high half).  A
 // code under 0x6400 is the f16 1024 + code, four bits further up 1024 + 16
 // code; the subtraction, the factor 1/16 and the product with a scale of 8
 // significant bits are all exact.
-__device__ __forceinline__ void unpack8(uint32_t w, const h16x2 scale, uint32_t (&out)[4])
+__device__ __forceinline__ void unpack8(const Unpack &u, uint32_t w, const h16x2 scale, uint32_t (&out)[4])
 {
     const h16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const h16x2 m0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, m1 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const uint32_t w8 = w >> 8;
-    const h16x2 c0 = as_h2((w & 0x000F000Fu) | 0x64006400u) + m0;
-    const h16x2 c1 = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, m1);
-    const h16x2 c2 = as_h2((w8 & 0x000F000Fu) | 0x64006400u) + m0;
-    const h16x2 c3 = __builtin_elementwise_fma(as_h2((w8 & 0x00F000F0u) | 0x64006400u), sixteenth, m1);
+    const h16x2 c0 = as_h2((w & u.low) | u.one) + m0;
+    const h16x2 c1 = __builtin_elementwise_fma(as_h2((w & u.high) | u.one), sixteenth, m1);
+    const h16x2 c2 = as_h2((w8 & u.low) | u.one) + m0;
+    const h16x2 c3 = __builtin_elementwise_fma(as_h2((w8 & u.high) | u.one), sixteenth, m1);
     out[0] = as_u(c0 * scale);
     out[1] = as_u(c1 * scale);
     out[2] = as_u(c2 * scale);
@@ -541,23 +550,51 @@ __device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnT
     return true;
 }
 
-// The last position that a column sees is len - n + row; keys [lo, hi) are
-// what the tile's columns see at all.
-__device__ __forceinline__ void tile_keys(const AttnTile &t, int group, int window, int W, int &minpos, int &maxpos,
-                                          int &lo, int &hi)
+// The last position that a column sees is len - n + row; minpos and maxpos are
+// the first and last column's, and pages pg0 .. pg0 + pages - 1 hold all that
+// the tile's columns see (as far as the table has columns).
+__device__ __forceinline__ void tile_pages(const Kv4Attn &a, const AttnTile &t, int W, int &minpos, int &maxpos, int &pg0,
+                                           int &pages)
 {
-    minpos = t.len - t.n + t.cb / group;
-    maxpos = t.len - t.n + min(t.cb + W - 1, t.ncols - 1) / group;
-    hi = maxpos + 1;
-    lo = window ? max(0, minpos - window + 1) : 0;
+    minpos = t.len - t.n + t.cb / a.group;
+    maxpos = t.len - t.n + min(t.cb + W - 1, t.ncols - 1) / a.group;
+    const int lo = a.window ? max(0, minpos - a.window + 1) : 0;
+    pg0 = lo / KV4_PAGE;
+    pages = maxpos < lo ? 0 : max(min(maxpos / KV4_PAGE + 1, a.max_pages) - pg0, 0);
+}
+
+// Workgroups that share a tile of so many pages: `chunk` pages each, the last
+// of `splits` what is left.  The sequence's own length says how many, so that
+// a long one among short ones is not one workgroup's work.
+__device__ __forceinline__ int tile_parts(int pages, int chunk, int splits)
+{
+    return max(1, min((pages + chunk - 1) / chunk, splits));
 }
 
 // One page's block as a wave holds it: lane l = (r, kg) = (l % 16, l / 16) has
 // of K rows 4r + t (t = 0..3) the D / 4 columns from kg D / 4, of V positions
 // 16 kg .. 16 kg + 15 of the D / 16 columns from r D / 16, and their scales.
 template <int D>
-struct PageRegs {
-    uint32_t k[4][D / 32], v[4][D / 32], ks[2], vs[8];
+struct PageK {
+    uint32_t k[4][D / 32], s[2];
+};
+template <int D>
+struct PageV {
+    uint32_t v[4][D / 32], s[8];
+};
+
+// Where a lane's parts lie in a block, apart from what is the same for all
+// lanes: 32 bits beside a scalar address, one register each.
+template <int D>
+struct LaneAt {
+    uint32_t k, ks, v, vs;
+    __device__ __forceinline__ LaneAt(int r, int kg)
+    {
+        k = kv4_k_at(D, 4 * r) + kg * (D / 8);
+        ks = kv4_ks_at(D, 4 * r, kg * (D / 4) / 32);
+        v = kv4_v_at(D, 16 * kg, r * (D / 64));
+        vs = kv4_vs_at(D, 16 * kg, r * (D / 16) / 32);
+    }
 };
 
 template <int D>
@@ -567,25 +604,29 @@ __device__ __forceinline__ void load_words(uint32_t *out, const uint8_t *p)
         const u32x4 w = *(const u32x4 *)p;
         out[0] = w.x, out[1] = w.y, out[2] = w.z, out[3] = w.w;
     } else {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 w = *(const u32x2 *)p;
+        const uint2 w = *(const uint2 *)p;
         out[0] = w.x, out[1] = w.y;
     }
 }
 
 template <int D>
-__device__ __forceinline__ void load_page(PageRegs<D> &g, const uint8_t *blk, int r, int kg)
+__device__ __forceinline__ void load_page(PageK<D> &g, const uint8_t *blk, const LaneAt<D> &at)
 {
 #pragma unroll
-    for (int t = 0; t < 4; t++) load_words<D>(g.k[t], blk + kv4_k_at(D, 4 * r + t) + kg * (D / 8));
-    const uint2 ks = *(const uint2 *)(blk + kv4_ks_at(D, 4 * r, kg * (D / 4) / 32));
-    g.ks[0] = ks.x, g.ks[1] = ks.y;
+    for (int t = 0; t < 4; t++) load_words<D>(g.k[t], blk + t * (kv4_k_at(D, 1) - kv4_k_at(D, 0)) + at.k);
+    const uint2 s = *(const uint2 *)(blk + at.ks);
+    g.s[0] = s.x, g.s[1] = s.y;
+}
+
+template <int D>
+__device__ __forceinline__ void load_page(PageV<D> &g, const uint8_t *blk, const LaneAt<D> &at)
+{
 #pragma unroll
-    for (int q = 0; q < 4; q++) load_words<D>(g.v[q], blk + kv4_v_at(D, 16 * kg + 4 * q, r * (D / 64)));
-    const u32x4 *vs = (const u32x4 *)(blk + kv4_vs_at(D, 16 * kg, r * (D / 16) / 32));
-    const u32x4 v0 = vs[0], v1 = vs[1];
-    g.vs[0] = v0.x, g.vs[1] = v0.y, g.vs[2] = v0.z, g.vs[3] = v0.w;
-    g.vs[4] = v1.x, g.vs[5] = v1.y, g.vs[6] = v1.z, g.vs[7] = v1.w;
+    for (int q = 0; q < 4; q++) load_words<D>(g.v[q], blk + q * (kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0)) + at.v);
+    const u32x4 *s = (const u32x4 *)(blk + at.vs);
+    const u32x4 s0 = s[0], s1 = s[1];
+    g.s[0] = s0.x, g.s[1] = s0.y, g.s[2] = s0.z, g.s[3] = s0.w;
+    g.s[4] = s1.x, g.s[5] = s1.y, g.s[6] = s1.z, g.s[7] = s1.w;
 }
 
 // A column's query as the second operand of K q: its D / 4 values from kg D /
@@ -641,51 +682,55 @@ struct Running {
     f32x4 o[D / 16] = {};
 };
 
-// One page: scores of 64 keys (lane (m, kg): keys 16 kg + 4 i + t), the running
-// softmax, and P V on the same lanes, with no exchange between lanes but the
-// maximum's.
+// Scores of one page's 64 keys: lane (m, kg) gets column m's of keys 16 kg + 4 i
+// + t as x[t][i].
 template <class T, int D>
-__device__ __forceinline__ void page_step(Running<D> &s, const PageRegs<D> &g, const Query<T, D> &q, float unit,
-                                          bool edge, int key0, int pos, int window, int len, int kg)
+__device__ __forceinline__ void page_scores(f32x4 (&x)[4], const Unpack &un, const PageK<D> &g, const Query<T, D> &q)
 {
-    constexpr int PARTS = Query<T, D>::PARTS;
-    f32x4 x[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        const uint32_t sc = g.ks[t / 2];
+        const uint32_t sc = g.s[t / 2];
         const uint32_t both = t % 2 ? (sc >> 16) | (sc & 0xFFFF0000u) : (sc & 0xFFFFu) | (sc << 16);
         f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < D / 32; j++) {
             uint32_t a[4];
-            unpack8(g.k[t][j], as_h2(both), a);
+            unpack8(un, g.k[t][j], as_h2(both), a);
             const half8 k8 = as_half8(a[0], a[1], a[2], a[3]);
-            if constexpr (PARTS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q.f[1][j], acc, 0, 0, 0);
+            if constexpr (Query<T, D>::PARTS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q.f[1][j], acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q.f[0][j], acc, 0, 0, 0);
         }
         x[t] = acc;
     }
-    uint32_t vs[8];
+}
+
+// The page at an edge: keys that a column does not see, and values past the
+// sequence's end, which may hold anything, count as zero (0 * NaN is not 0).
+template <int D>
+__device__ __forceinline__ void page_edge(f32x4 (&x)[4], PageV<D> &g, int key0, int pos, int window, int len, int kg)
+{
+    const int first = key0 + 16 * kg;
+    const int low = window ? pos - window : -1;
 #pragma unroll
-    for (int i = 0; i < 8; i++) vs[i] = g.vs[i];
-    if (edge) {
-        // keys that a column does not see; values past the sequence's end,
-        // which may hold anything, count as zero (0 * NaN is not 0)
-        const int first = key0 + 16 * kg;
-        const int low = window ? pos - window : -1;
+    for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int key = first + 4 * i + t;
-                if (key > pos || key <= low) x[t][i] = -INFINITY;
-            }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int left = len - (first + 2 * i);
-            vs[i] = left <= 0 ? 0u : left == 1 ? vs[i] & 0xFFFFu : vs[i];
+        for (int i = 0; i < 4; i++) {
+            const int key = first + 4 * i + t;
+            if (key > pos || key <= low) x[t][i] = -INFINITY;
         }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int left = len - (first + 2 * i);
+        g.s[i] = left <= 0 ? 0u : left == 1 ? g.s[i] & 0xFFFFu : g.s[i];
     }
+}
+
+// The running softmax, and P V on the lanes that hold the scores: nothing goes
+// from lane to lane but the maximum.
+template <class T, int D>
+__device__ __forceinline__ void page_values(Running<D> &s, const Unpack &un, f32x4 (&x)[4], const PageV<D> &g, float unit)
+{
+    constexpr int PARTS = Query<T, D>::PARTS;
     float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; t++) top = fmaxf(top, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
@@ -718,7 +763,7 @@ __device__ __forceinline__ void page_step(Running<D> &s, const PageRegs<D> &g, c
         for (int c = 0; c < D / 64; c++) {       // units of four columns
             uint32_t a[4][4];
 #pragma unroll
-            for (int h = 0; h < 4; h++) unpack8(g.v[2 * u + h / 2][2 * c + h % 2], as_h2(vs[4 * u + h]), a[h]);
+            for (int h = 0; h < 4; h++) unpack8(un, g.v[2 * u + h / 2][2 * c + h % 2], as_h2(g.s[4 * u + h]), a[h]);
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 const half8 v8 = as_half8(a[0][n], a[1][n], a[2][n], a[3][n]);
@@ -744,11 +789,11 @@ k_kv4_attn(Kv4Attn a)
     const int ti = blockIdx.x, sp = blockIdx.y, hk = blockIdx.z;
     AttnTile t;
     if (!find_tile(a, ti, W, t)) return;
-    int minpos, maxpos, lo, hi;
-    tile_keys(t, a.group, a.window, W, minpos, maxpos, lo, hi);
-    const int pg0 = lo / KV4_PAGE, pg1 = min((hi + KV4_PAGE - 1) / KV4_PAGE, a.max_pages);
-    const int pages = hi > lo ? max(pg1 - pg0, 0) : 0;
-    const int pb = pg0 + (int)((int64_t)pages * sp / a.splits), pe = pg0 + (int)((int64_t)pages * (sp + 1) / a.splits);
+    int minpos, maxpos, pg0, pages;
+    tile_pages(a, t, W, minpos, maxpos, pg0, pages);
+    const int parts = tile_parts(pages, a.chunk, a.splits);
+    if (sp >= parts) return;
+    const int pb = pg0 + sp * a.chunk, pe = sp == parts - 1 ? pg0 + pages : pb + a.chunk;
 
     const int cc = t.cb + r, row = cc / a.group;
     const bool valid = cc < t.ncols;
@@ -768,26 +813,42 @@ k_kv4_attn(Kv4Attn a)
     Running<D> s;
     bool poisoned = pos >= (int64_t)a.max_pages * KV4_PAGE;   // sees a page that the table has no column for
     const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
-    for (int base = pb + wave; base < pe; base += 256) {
-        // 64 of this wave's pages: one id a lane
-        const int mine = base + 4 * lane;
-        const int id = mine < pe ? table[mine] : -1;
-        const int count = min(64, (pe - base + 3) / 4);
-        for (int i = 0; i < count; i++) {
-            const int page = base + 4 * i;
-            const int pid = __builtin_amdgcn_readlane(id, i);
-            const bool bad = pid < 0 || pid >= a.cache.n_pages;
-            if (bad) {               // what sees this page is NaN
-                const int first = page * KV4_PAGE;
-                poisoned |= pos >= first && (!a.window || pos - a.window < first + KV4_PAGE - 1);
-                continue;
+    const Unpack un;
+    const LaneAt<D> at(r, kg);
+    const int n = (pe - pb - wave + 3) / 4;      // this wave's pages: pb + wave + 4 i
+    int i = -1, page = 0, ids = 0;               // ids: of 64 of them, one a lane
+    const uint8_t *blk = nullptr;
+    const auto next = [&] {
+        while (++i < n) {
+            page = pb + wave + 4 * i;
+            if ((i & 63) == 0) ids = page + 4 * lane < pe ? table[page + 4 * lane] : -1;
+            const int id = __builtin_amdgcn_readlane(ids, i & 63);
+            if (id >= 0 && id < a.cache.n_pages) {
+                blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
+                return true;
             }
-            PageRegs<D> g;
-            load_page<D>(g, a.cache.base + pid * a.cache.stride + (int64_t)hk * kv4_block(D), r, kg);
-            const int key0 = page * KV4_PAGE;
-            const bool edge = key0 + KV4_PAGE - 1 > minpos || (a.window && key0 <= maxpos - a.window);
-            page_step<T, D>(s, g, q, unit, edge, key0, pos, a.window, t.len, kg);
+            const int first = page * KV4_PAGE;   // what sees this page is NaN
+            poisoned |= pos >= first && (!a.window || pos - a.window < first + KV4_PAGE - 1);
         }
+        return false;
+    };
+    // V is on its way while K is multiplied, the next page's K while V is
+    PageK<D> gk;
+    bool more = next();
+    if (more) load_page(gk, blk, at);
+    while (more) {
+        PageV<D> gv;
+        load_page(gv, blk, at);
+        const int key0 = page * KV4_PAGE;
+        f32x4 x[4];
+        __builtin_amdgcn_sched_barrier(0);
+        page_scores<T, D>(x, un, gk, q);
+        __builtin_amdgcn_sched_barrier(0);
+        more = next();
+        if (more) load_page(gk, blk, at);
+        if (key0 + KV4_PAGE - 1 > minpos || (a.window && key0 <= maxpos - a.window))
+            page_edge<D>(x, gv, key0, pos, a.window, t.len, kg);
+        page_values<T, D>(s, un, x, gv, unit);
     }
     s.l = add_xor32(add_xor16(s.l));
     if (poisoned) s.l = __builtin_nanf("");
@@ -803,8 +864,8 @@ k_kv4_attn(Kv4Attn a)
                 f32x4{s.o[i][e], s.o[i + 1][e], s.o[i + 2][e], s.o[i + 3][e]} * f;
     __syncthreads();
     const int64_t pi = ((int64_t)ti * a.cache.heads + hk) * a.splits + sp;
-    for (int i = threadIdx.x; i < W * D / 4; i += 256) {
-        const int c = i / (D / 4), d = i % (D / 4) * 4, col = t.cb + c;
+    for (int e = threadIdx.x; e < W * D / 4; e += 256) {
+        const int c = e / (D / 4), d = e % (D / 4) * 4, col = t.cb + c;
         if (col >= t.ncols) break;
         f32x4 o = {0, 0, 0, 0};
         float l = 0.0f;
@@ -814,7 +875,7 @@ k_kv4_attn(Kv4Attn a)
             o += *(const f32x4 *)&so[w][c][d];
             l += sm[w][c] == -INFINITY ? 0.0f * sl[w][c] : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - Mc);
         }
-        if (a.splits > 1) {
+        if (parts > 1) {
             if (d == 0) a.part[pi * 32 + c] = Mc, a.part[pi * 32 + 16 + c] = l;
             *(f32x4 *)(a.part + a.part_rows + (pi * W + c) * D + d) = o;
         } else {
@@ -825,8 +886,8 @@ k_kv4_attn(Kv4Attn a)
     }
 }
 
-// The splits of one column joined: weights 2^(m - M), then the rows' weighted
-// sum, 256 / (D / 4) of them at a time.
+// The parts of a tile's columns joined, one column at a time: weights 2^(m - M),
+// then the rows' weighted sum, 256 / (D / 4) of them at once.
 template <class T, int D>
 __global__ void __launch_bounds__(256)
 k_kv4_attn_join(Kv4Attn a)
@@ -834,44 +895,51 @@ k_kv4_attn_join(Kv4Attn a)
     constexpr int L = D / 4, ROWS = 256 / L;
     __shared__ float w[64];
     __shared__ f32x4 so[ROWS][L];
-    const int ti = blockIdx.x, c = blockIdx.y, hk = blockIdx.z, lane = threadIdx.x & 63;
+    const int ti = blockIdx.x, hk = blockIdx.z, lane = threadIdx.x & 63;
     AttnTile t;
     if (!find_tile(a, ti, KV4_W, t)) return;
-    const int col = t.cb + c;
-    if (col >= t.ncols) return;
+    int minpos, maxpos, pg0, pages;
+    tile_pages(a, t, KV4_W, minpos, maxpos, pg0, pages);
+    const int parts = tile_parts(pages, a.chunk, a.splits);
+    if (parts == 1) return;
     const int64_t p0 = ((int64_t)ti * a.cache.heads + hk) * a.splits;
-    float m = -INFINITY, l = 0.0f;
-    if (lane < a.splits) m = a.part[(p0 + lane) * 32 + c], l = a.part[(p0 + lane) * 32 + 16 + c];
-    const float M = wave_max_dpp(m);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-    const float sum = wave_sum_dpp(l * f);
-    if (threadIdx.x < 64) w[lane] = f;
-    __syncthreads();
     const int i = threadIdx.x % L, g = threadIdx.x / L;
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = g; s < a.splits; s += ROWS)
-        o += *(const f32x4 *)(a.part + a.part_rows + ((p0 + s) * KV4_W + c) * D + 4 * i) * w[s];
-    so[g][i] = o;
-    __syncthreads();
-    if (g) return;
+    for (int c = blockIdx.y; c < min(KV4_W, t.ncols - t.cb); c += gridDim.y) {
+        const int col = t.cb + c;
+        float m = -INFINITY, l = 0.0f;
+        if (lane < parts) m = a.part[(p0 + lane) * 32 + c], l = a.part[(p0 + lane) * 32 + 16 + c];
+        const float M = wave_max_dpp(m);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+        const float sum = wave_sum_dpp(l * f);
+        __syncthreads();             // the column before is read
+        if (threadIdx.x < 64) w[lane] = f;
+        __syncthreads();
+        f32x4 o = {0, 0, 0, 0};
+        for (int s = g; s < parts; s += ROWS)
+            o += *(const f32x4 *)(a.part + a.part_rows + ((p0 + s) * KV4_W + c) * D + 4 * i) * w[s];
+        so[g][i] = o;
+        __syncthreads();
+        if (g) continue;
 #pragma unroll
-    for (int k = 1; k < ROWS; k++) o += so[k][i];
-    store4((T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + 4 * i,
-           sum == 0.0f ? f32x4{0, 0, 0, 0} : o / sum, a.vec);
+        for (int k = 1; k < ROWS; k++) o += so[k][i];
+        store4((T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + 4 * i,
+               sum == 0.0f ? f32x4{0, 0, 0, 0} : o / sum, a.vec);
+    }
 }
 
 // Tiles there can be: the number after the last sequence's last.
 static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return kv4_first_tile(rows, group, n_seqs, W); }
 
-// Shares that the pages of each tile are cut into: enough workgroups to fill
-// the card, at least a page for each of their waves.
-int kv4_attn_splits(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
+// Pages that a workgroup takes, and the most workgroups of a tile.
+void kv4_attn_split(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window, int *chunk, int *splits)
 {
     const int64_t items = attn_tiles(rows, n_seqs, group, KV4_W) * kv_heads;
     int64_t pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
     if (window) pages = std::min<int64_t>(pages, (window + KV4_W - 2) / KV4_PAGE + 2);
-    const int64_t want = std::min((1024 + items - 1) / std::max<int64_t>(items, 1), (pages + 3) / 4);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
+    int64_t per = std::max<int64_t>(items * pages / 1024, (pages + 63) / 64);
+    per = std::max<int64_t>((per + 3) / 4 * 4, 4);
+    *chunk = (int)std::min<int64_t>(per, INT32_MAX / KV4_PAGE);
+    *splits = (int)std::max<int64_t>(1, (pages + per - 1) / per);
 }
 
 template <class T, int D>
@@ -881,7 +949,9 @@ static hipError_t launch_attn(const Kv4Attn &a, hipStream_t s)
     hipLaunchKernelGGL((k_kv4_attn<T, D>), dim3(tiles, a.splits, a.cache.heads), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL((k_kv4_attn_join<T, D>), dim3(tiles, KV4_W, a.cache.heads), dim3(256), 0, s, a);
+    // a workgroup a column of an average sequence's tile
+    const int64_t cols = std::min<int64_t>(KV4_W, ((int64_t)a.rows * a.group + a.n_seqs - 1) / a.n_seqs);
+    hipLaunchKernelGGL((k_kv4_attn_join<T, D>), dim3(tiles, (unsigned)cols, a.cache.heads), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

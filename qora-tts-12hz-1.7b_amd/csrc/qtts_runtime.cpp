@@ -2100,22 +2100,25 @@ static int check_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a)
     return QTTS_OK;
 }
 
-static int attention_splits(const qtts_kv4_attention_args *a)
+// How a call's pages are split, and the parts whose results the workspace holds
+// (0: nothing is split).
+struct AttnSplit { int chunk, splits; int64_t parts; };
+static AttnSplit attention_split(const qtts_kv4_attention_args *a)
 {
-    return kv4_attn_splits(a->rows, a->n_seqs, a->n_heads / a->cache->n_kv_heads, a->cache->n_kv_heads, a->max_len, a->window);
+    const int group = a->n_heads / a->cache->n_kv_heads;
+    AttnSplit s{};
+    kv4_attn_split(a->rows, a->n_seqs, group, a->cache->n_kv_heads, a->max_len, a->window, &s.chunk, &s.splits);
+    if (s.splits > 1 && a->rows && a->n_seqs)
+        s.parts = kv4_first_tile(a->rows, group, a->n_seqs, KV4_W) * a->cache->n_kv_heads * s.splits;
+    return s;
 }
-
-// Floats of the partial results: maxima and sums, then rows.
-static int64_t attention_parts(const qtts_kv4_attention_args *a)
-{
-    return kv4_first_tile(a->rows, a->n_heads / a->cache->n_kv_heads, a->n_seqs, KV4_W) * a->cache->n_kv_heads * attention_splits(a);
-}
+static int64_t parts_bytes(const qtts_kv4_attention_args *a, int64_t parts) { return parts * (32 + KV4_W * a->cache->head_dim) * 4; }
 
 extern "C" int qtts_kv4_attention_workspace(const qtts_kv4_attention_args *a, int64_t *bytes)
 {
     if (!a || !bytes) return QTTS_ERR_INVALID;
     RCHK(check_kv4_attention(nullptr, a));
-    *bytes = a->rows && a->n_seqs && attention_splits(a) > 1 ? attention_parts(a) * (32 + KV4_W * a->cache->head_dim) * 4 : 0;
+    *bytes = parts_bytes(a, attention_split(a).parts);
     return QTTS_OK;
 }
 
@@ -2123,8 +2126,8 @@ extern "C" int qtts_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a,
 {
     if (!a || (!c && !(flags & QTTS_CHECK_ONLY))) return QTTS_ERR_INVALID;
     RCHK(check_kv4_attention(c, a));
-    int64_t need = 0;
-    RCHK(qtts_kv4_attention_workspace(a, &need));
+    const AttnSplit split = attention_split(a);
+    const int64_t need = parts_bytes(a, split.parts);
     if (need > a->workspace_bytes || (need && !a->workspace) || (need && !kv4_aligned(a->workspace, 16)))
         return fail(c, QTTS_ERR_CAPACITY, "workspace of %lld bytes, 16-byte aligned, needed; %lld given", (long long)need,
                     (long long)a->workspace_bytes);
@@ -2141,8 +2144,8 @@ extern "C" int qtts_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a,
     k.row_start = a->row_start, k.lengths = a->lengths, k.table = a->table, k.table_stride = a->table_stride;
     k.part = (float *)a->workspace;
     k.rows = (int32_t)a->rows, k.n_seqs = a->n_seqs, k.max_pages = a->max_pages, k.group = a->n_heads / a->cache->n_kv_heads;
-    k.window = a->window, k.splits = attention_splits(a), k.scale = a->scale;
-    k.part_rows = 32 * attention_parts(a);
+    k.window = a->window, k.chunk = split.chunk, k.splits = split.splits, k.scale = a->scale;
+    k.part_rows = 32 * split.parts;
     k.vec = moves4(a->q, a->q_stride, a->dtype) && moves4(a->out, a->out_stride, a->dtype);
     DeviceGuard guard(c->device);
     return kv4_done(c, enqueue_kv4_attn(k, a->dtype, (int)D, (hipStream_t)stream));
