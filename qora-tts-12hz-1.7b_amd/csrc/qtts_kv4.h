@@ -58,7 +58,7 @@ struct Kv4Attn {
     Kv4Pages cache;
     const int32_t *row_start, *lengths, *table;
     int64_t table_stride;
-    float *part;                     // splits > 1: [tile][kv head][split] {16 maxima, 16 sums}, then the rows
+    float *part;                     // splits > 1: [tile][kv head][split] {W maxima, W sums}, then the rows
     int64_t part_rows;               // floats before the rows
     int32_t rows, n_seqs, max_pages, group;
     int32_t window, chunk, splits;   // pages of a workgroup, most workgroups of a tile
@@ -67,17 +67,23 @@ struct Kv4Attn {
 };
 
 // The work of a sequence is cut into tiles of W columns, a column being a
-// (row, query head of the kv head) pair in that order.  Tile numbers are
-// found without a sum over the sequences: sequence b's first tile is
-// row_start[b] * group / W + b, since a sequence of c columns starting at
-// column s needs at most (s + c) / W - s / W + 1 tiles.
-constexpr int KV4_W = 16;
+// (row, query head of the kv head) pair in that order.  A tile's number is found
+// without a sum over all sequences: blocks of 64 sequences begin at tile
+// row_start[b] * group / W + b, since c columns starting at column s need at most
+// (s + c) / W - s / W + 1 tiles; within a block tiles are numbered without gaps
+// (numbers that no tile has, spread evenly among the others, left the card half
+// idle: workgroups go round XCDs and their parts by number).
+constexpr int KV4_W = 16, KV4_WIDE = 128;
 __host__ __device__ constexpr int64_t kv4_first_tile(int64_t row, int group, int b, int W) { return row * group / W + b; }
 
 hipError_t enqueue_kv4_tables(const Kv4Tables &a, hipStream_t s);
 hipError_t enqueue_qk_norm_rope(const QkNormRope &a, int dtype, int D, bool store, hipStream_t s);
 hipError_t enqueue_kv4_gather(const Kv4Pages &c, int D, const int64_t *slots, int n, int dtype, void *K, void *V, hipStream_t s);
-void kv4_attn_split(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window, int *chunk, int *splits);
-hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, hipStream_t s);
+struct Kv4Cut {
+    int width, chunk, splits;
+    int64_t parts;                   // partial results that the workspace holds; 0: nothing is split
+};
+Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window);
+hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, int width, hipStream_t s);
 
 }  // namespace qtts

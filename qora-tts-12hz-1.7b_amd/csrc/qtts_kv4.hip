@@ -207,6 +207,17 @@ __device__ __forceinline__ double lanes_sum(double v)
     return v;
 }
 
+// 1 / sqrt(x): within an ulp in f32; in f64 from the instruction's 2^-28 or so by
+// two steps of Newton's (each squares the error).
+__device__ __forceinline__ float inv_sqrt(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inv_sqrt(double x)
+{
+    double r = __builtin_amdgcn_rsq(x);
+    const double h = 0.5 * x;
+    r = fma(r, fma(-h * r, r, 0.5), r);
+    return fma(r, fma(-h * r, r, 0.5), r);
+}
+
 // One lane's part of a head: columns 4j .. 4j+3 and, D / 2 further, the ones
 // they are rotated with.
 template <class F>
@@ -224,9 +235,9 @@ __device__ __forceinline__ void norm_rope(Head<F> &x, bool norm, f32x4 ga, f32x4
     if (norm) {
         F ss = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+        for (int i = 0; i < 4; i++) ss = fma(x.a[i], x.a[i], fma(x.b[i], x.b[i], ss));
         ss = lanes_sum<L>(ss);
-        const F r = F(1) / (F)sqrt(ss * F(1.0 / (8 * L)) + (F)eps);
+        const F r = inv_sqrt(ss * F(1.0 / (8 * L)) + (F)eps);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x.a[i] = x.a[i] * r * (F)ga[i];
@@ -244,134 +255,177 @@ __device__ __forceinline__ void norm_rope(Head<F> &x, bool norm, f32x4 ga, f32x4
 
 // Codes and scale of 32 values, four in each of eight neighbouring lanes: the
 // step is -1/8 of the value of largest magnitude, rounded to f16 and then to
-// 8 significant bits; the nearest step's number, halves to even, plus 8.  The
-// quotient is a product with the reciprocal except next to a half, where only
-// the division says on which side it lies.
-__device__ __forceinline__ uint32_t quantise(const double (&x)[4], uint16_t &scale)
+// 8 significant bits; the nearest step's number, halves to even, plus 8.
+//
+// In f32 where that decides as f64 does, else in f64: rounding to f32 keeps the
+// order of values, so only two extremes that it makes equal have to be looked at
+// again, and the quotient (at most 16, off by 2^-22 of it from x, the reciprocal
+// and the product) only next to a half.  In f64 throughout, the quantisation of
+// 4001 rows of 16 heads took 22 us instead of TIME.
+template <class F>
+__device__ __forceinline__ uint32_t quantise(const F (&x)[4], uint16_t &scale)
 {
-    double v[4], hi, lo;
+    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = fmin(fmax(x[i], -65280.0), 65280.0);
-    hi = fmax(fmax(v[0], v[1]), fmax(v[2], v[3]));
-    lo = fmin(fmin(v[0], v[1]), fmin(v[2], v[3]));
-    hi = fmax(hi, dpp_mov64<0xB1>(hi)), lo = fmin(lo, dpp_mov64<0xB1>(lo));
-    hi = fmax(hi, dpp_mov64<0x4E>(hi)), lo = fmin(lo, dpp_mov64<0x4E>(lo));
-    hi = fmax(hi, dpp_mov64<0x141>(hi)), lo = fmin(lo, dpp_mov64<0x141>(lo));
-    const _Float16 h = (_Float16)(float)((hi >= -lo ? hi : lo) * -0.125);
-    scale = (uint16_t)((__builtin_bit_cast(uint16_t, h) + 4) & 0xFFF8);
-    const double d = (double)(float)__builtin_bit_cast(_Float16, scale);
-    const double inv = d != 0.0 ? 1.0 / d : 0.0;
-    uint32_t codes = 0;
+    for (int i = 0; i < 4; i++) v[i] = (float)x[i];
+    float hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+    hi = fmaxf(hi, dpp_mov<0xB1>(hi)), lo = fminf(lo, dpp_mov<0xB1>(lo));
+    hi = fmaxf(hi, dpp_mov<0x4E>(hi)), lo = fminf(lo, dpp_mov<0x4E>(lo));
+    hi = fmaxf(hi, dpp_mov<0x141>(hi)), lo = fminf(lo, dpp_mov<0x141>(lo));
+    // beyond the format's range a value's quotient goes past the last code, where it ends
+    hi = fminf(hi, 65280.0f), lo = fmaxf(lo, -65280.0f);
+    bool plus = hi >= -lo;
+    if constexpr (std::is_same<F, double>::value)
+        if (__any(hi == -lo && hi != 0.0f)) {
+            double h = fmax(fmax(x[0], x[1]), fmax(x[2], x[3])), l = fmin(fmin(x[0], x[1]), fmin(x[2], x[3]));
+            h = fmax(h, dpp_mov64<0xB1>(h)), l = fmin(l, dpp_mov64<0xB1>(l));
+            h = fmax(h, dpp_mov64<0x4E>(h)), l = fmin(l, dpp_mov64<0x4E>(l));
+            h = fmax(h, dpp_mov64<0x141>(h)), l = fmin(l, dpp_mov64<0x141>(l));
+            plus = fmin(h, 65280.0) >= -fmax(l, -65280.0);
+        }
+    const _Float16 d16 = (_Float16)((plus ? hi : lo) * -0.125f);
+    scale = (uint16_t)((__builtin_bit_cast(uint16_t, d16) + 4) & 0xFFF8);
+    const float d = (float)__builtin_bit_cast(_Float16, scale);
+    const float inv = d != 0.0f ? __builtin_amdgcn_rcpf(d) : 0.0f;
+    float code[4], far = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double q = v[i] * inv;
-        double r = rint(q);
-        if (fabs(fabs(q - r) - 0.5) < 1e-9) r = rint(v[i] / d);
-        codes |= (uint32_t)(int)fmin(fmax(r + 8.0, 0.0), 15.0) << (4 * i);
+        const float q = v[i] * inv, r = __builtin_rintf(q);
+        far = fmaxf(far, fabsf(q - r));
+        code[i] = __builtin_amdgcn_fmed3f(r + 8.0f, 0.0f, 15.0f);
     }
-    return codes;
+    if (far > 0.49999f) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double q = fmin(fmax((double)x[i], -65280.0), 65280.0) / (double)d;
+            code[i] = (float)fmin(fmax(rint(q) + 8.0, 0.0), 15.0);
+        }
+    }
+    return (uint32_t)fmaf(4096.0f, code[3], fmaf(256.0f, code[2], fmaf(16.0f, code[1], code[0])));
 }
 
 // D / 8 lanes take one row's query heads of one kv head, that kv head's key
 // and, with a cache, its value: the angles are loaded once for all of them.
-// Bound by memory: rows in, q out and 4.5 bits a value into the pages.
-template <class T, int D, bool STORE>
+// ONE_ROW: a wave's heads are of one row (the kv heads are a multiple of those
+// that a wave holds), whose addresses are then scalar.
+template <class T, int D, bool STORE, bool ONE_ROW>
 __global__ void __launch_bounds__(256)
 k_qk_norm_rope(QkNormRope a)
 {
-    constexpr int L = D / 8;
-    const int j = threadIdx.x % L;
-    const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (item >= (int64_t)a.rows * a.kv_heads) return;
-    const int row = (int)(item / a.kv_heads), hk = (int)(item % a.kv_heads);
-    const int32_t pos = a.positions ? a.positions[row] : 0;
-    if (pos < 0) return;
+    constexpr int L = D / 8, HEADS = 64 / L;
+    const int lane = threadIdx.x & 63, j = lane % L;
+    const int first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * HEADS;
+    int row, hk;
+    if constexpr (ONE_ROW) {
+        row = __builtin_amdgcn_readfirstlane(first / a.kv_heads);
+        hk = first - row * a.kv_heads + lane / L;
+    } else {
+        row = (first + lane / L) / a.kv_heads;
+        hk = (first + lane / L) % a.kv_heads;
+    }
+    if (row >= a.rows) return;
     const bool vec = a.vec;
-    const int at = 4 * j, up = D / 2 + 4 * j;    // a lane's columns
+    const uint32_t at = hk * D + 4 * j, up = at + D / 2;     // a lane's columns of k and v
+    const int32_t pos = a.positions ? a.positions[row] : 0;
 
-    const T *kp = (const T *)a.k + row * a.k_stride + hk * D;
+    // the loads that wait for nothing first
+    const T *kp = (const T *)a.k + row * a.k_stride;
     const f32x4 ka = load4(kp + at, vec), kb = load4(kp + up, vec);
     f32x4 va{}, vb{};
+    int64_t slot = 0;
     if constexpr (STORE) {
-        const T *vp = (const T *)a.v + row * a.v_stride + hk * D;
+        const T *vp = (const T *)a.v + row * a.v_stride;
         va = load4(vp + at, vec), vb = load4(vp + up, vec);
+        slot = a.slots[row];
     }
+    const T *qp = (const T *)a.q + row * a.q_stride;
+    const uint32_t qat = hk * a.group * D + 4 * j;
+    f32x4 qa = load4(qp + qat, vec), qb = load4(qp + (qat + D / 2), vec);
+    if (pos < 0) return;
     f32x4 c{}, s{};
     if (a.positions) {
         if (pos < a.max_pos) {
-            c = load4(a.cos + (int64_t)pos * (D / 2) + at, vec);
-            s = load4(a.sin + (int64_t)pos * (D / 2) + at, vec);
+            c = load4(a.cos + (int64_t)pos * (D / 2) + 4 * j, vec);
+            s = load4(a.sin + (int64_t)pos * (D / 2) + 4 * j, vec);
         } else {
             c = s = __builtin_nanf("");
         }
     }
 
     f32x4 ga{}, gb{};
-    if (a.q_norm) ga = load4((const _Float16 *)a.q_norm + at, vec), gb = load4((const _Float16 *)a.q_norm + up, vec);
+    if (a.q_norm) ga = load4((const _Float16 *)a.q_norm + 4 * j, vec), gb = load4((const _Float16 *)a.q_norm + D / 2 + 4 * j, vec);
+    T *qo = (T *)a.q_out + row * a.q_out_stride;
     for (int g = 0; g < a.group; g++) {
-        const int h = hk * a.group + g;
-        const T *qp = (const T *)a.q + row * a.q_stride + h * D;
-        const f32x4 qa = load4(qp + at, vec), qb = load4(qp + up, vec);
         Head<float> x;
 #pragma unroll
         for (int i = 0; i < 4; i++) x.a[i] = qa[i], x.b[i] = qb[i];
+        const uint32_t here = qat + g * D;
+        if (g + 1 < a.group) qa = load4(qp + (here + D), vec), qb = load4(qp + (here + D + D / 2), vec);
         norm_rope<float, L>(x, a.q_norm, ga, gb, a.eps, a.positions, c, s);
-        T *qo = (T *)a.q_out + row * a.q_out_stride + h * D;
-        store4(qo + at, f32x4{x.a[0], x.a[1], x.a[2], x.a[3]}, vec);
-        store4(qo + up, f32x4{x.b[0], x.b[1], x.b[2], x.b[3]}, vec);
+        store4(qo + here, f32x4{x.a[0], x.a[1], x.a[2], x.a[3]}, vec);
+        store4(qo + (here + D / 2), f32x4{x.b[0], x.b[1], x.b[2], x.b[3]}, vec);
     }
 
-    if (a.k_norm) ga = load4((const _Float16 *)a.k_norm + at, vec), gb = load4((const _Float16 *)a.k_norm + up, vec);
+    if (a.k_norm) ga = load4((const _Float16 *)a.k_norm + 4 * j, vec), gb = load4((const _Float16 *)a.k_norm + D / 2 + 4 * j, vec);
     using F = typename std::conditional<STORE, double, float>::type;
     Head<F> x;
 #pragma unroll
     for (int i = 0; i < 4; i++) x.a[i] = ka[i], x.b[i] = kb[i];
     norm_rope<F, L>(x, a.k_norm, ga, gb, a.eps, a.positions, c, s);
     if (a.k_out) {
-        T *ko = (T *)a.k_out + row * a.k_out_stride + hk * D;
+        T *ko = (T *)a.k_out + row * a.k_out_stride;
         store4(ko + at, f32x4{(float)x.a[0], (float)x.a[1], (float)x.a[2], (float)x.a[3]}, vec);
         store4(ko + up, f32x4{(float)x.b[0], (float)x.b[1], (float)x.b[2], (float)x.b[3]}, vec);
     }
     if constexpr (STORE) {
         bool nan = false;
-        double y[4], z[4];
+        float y[4], z[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             nan |= x.a[i] != x.a[i] || x.b[i] != x.b[i] || va[i] != va[i] || vb[i] != vb[i];
             y[i] = va[i], z[i] = vb[i];
         }
         // any lane of the head
-        const uint64_t lanes = ((1ull << L) - 1) << (threadIdx.x % 64 / L * L);
+        const uint64_t lanes = ((1ull << L) - 1) << (lane / L * L);
         nan = (__ballot(nan) & lanes) != 0;
         uint16_t s0, s1, s2, s3;
         const uint32_t k0 = quantise(x.a, s0), k1 = quantise(x.b, s1);
         const uint32_t v0 = quantise(y, s2), v1 = quantise(z, s3);
-        const int64_t slot = a.slots[row];
         if (slot < 0 || slot >= a.cache.n_pages * KV4_PAGE) return;
-        uint8_t *blk = a.cache.base + slot / KV4_PAGE * a.cache.stride + (int64_t)hk * kv4_block(D);
+        uint8_t *page = a.cache.base + slot / KV4_PAGE * a.cache.stride;
         const int p = (int)(slot % KV4_PAGE);
-        *(uint16_t *)(blk + kv4_k_at(D, p) + 2 * j) = (uint16_t)k0;
-        *(uint16_t *)(blk + kv4_k_at(D, p) + D / 4 + 2 * j) = (uint16_t)k1;
-        *(uint16_t *)(blk + kv4_v_at(D, p, j)) = (uint16_t)v0;
-        *(uint16_t *)(blk + kv4_v_at(D, p, j + D / 8)) = (uint16_t)v1;
+        const uint32_t blk = hk * kv4_block(D);
+        *(uint16_t *)(page + (blk + kv4_k_at(D, p) + 2 * j)) = (uint16_t)k0;
+        *(uint16_t *)(page + (blk + kv4_k_at(D, p) + D / 4 + 2 * j)) = (uint16_t)k1;
+        *(uint16_t *)(page + (blk + kv4_v_at(D, p, j))) = (uint16_t)v0;
+        *(uint16_t *)(page + (blk + kv4_v_at(D, p, j + D / 8))) = (uint16_t)v1;
         if (j % 8 == 0) {
-            *(uint16_t *)(blk + kv4_ks_at(D, p, j / 8)) = nan ? 0x7E00 : s0;
-            *(uint16_t *)(blk + kv4_ks_at(D, p, j / 8 + D / 64)) = nan ? 0x7E00 : s1;
-            *(uint16_t *)(blk + kv4_vs_at(D, p, j / 8)) = nan ? 0 : s2;
-            *(uint16_t *)(blk + kv4_vs_at(D, p, j / 8 + D / 64)) = nan ? 0 : s3;
+            *(uint16_t *)(page + (blk + kv4_ks_at(D, p, j / 8))) = nan ? 0x7E00 : s0;
+            *(uint16_t *)(page + (blk + kv4_ks_at(D, p, j / 8 + D / 64))) = nan ? 0x7E00 : s1;
+            *(uint16_t *)(page + (blk + kv4_vs_at(D, p, j / 8))) = nan ? 0 : s2;
+            *(uint16_t *)(page + (blk + kv4_vs_at(D, p, j / 8 + D / 64))) = nan ? 0 : s3;
         }
     }
+}
+
+template <class T, int D, bool ONE_ROW>
+static void launch_qk_as(const QkNormRope &a, bool store, hipStream_t s)
+{
+    const int64_t heads = (int64_t)a.rows * a.kv_heads, per = 256 / (D / 8);
+    const dim3 grid((unsigned)((heads + per - 1) / per));
+    if (store)
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, true, ONE_ROW>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, false, ONE_ROW>), grid, dim3(256), 0, s, a);
 }
 
 template <class T, int D>
 static hipError_t launch_qk(const QkNormRope &a, bool store, hipStream_t s)
 {
-    const int64_t groups = (int64_t)a.rows * a.kv_heads, per = 256 / (D / 8);
-    const dim3 grid((unsigned)((groups + per - 1) / per));
-    if (store)
-        hipLaunchKernelGGL((k_qk_norm_rope<T, D, true>), grid, dim3(256), 0, s, a);
+    if (a.kv_heads % (512 / D) == 0)
+        launch_qk_as<T, D, true>(a, store, s);
     else
-        hipLaunchKernelGGL((k_qk_norm_rope<T, D, false>), grid, dim3(256), 0, s, a);
+        launch_qk_as<T, D, false>(a, store, s);
     return hipGetLastError();
 }
 
@@ -520,34 +574,49 @@ struct AttnTile {
     int b, r0, n, len, cb, ncols;
 };
 
-// The tile with number ti, found by the whole wave: each round, 64 lanes look
-// at 64 evenly spaced sequences (one load of latency for 64 sequences, two
-// for 4096).  False where no tile has this number, and for row sums that
+// The tile with number ti, found by the whole wave: first its block of 64
+// sequences (each round, 64 lanes look at 64 evenly spaced ones), then the
+// sequence by a sum over the block's.  One load of latency for 64 sequences,
+// two for 4096.  False where no tile has this number, and for row sums that
 // are none.
 __device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnTile &t)
 {
     const int lane = threadIdx.x & 63;
-    int lo = 0, cnt = a.n_seqs;
+    const auto start = [&](int b) { return min(max(a.row_start[b], 0), a.rows); };
+    int lo = 0, cnt = (a.n_seqs + 63) / 64;
     while (cnt > 1) {
         const int step = (cnt + 63) / 64, i = lane * step;
-        const bool in = i < cnt && kv4_first_tile(min(max(a.row_start[lo + i], 0), a.rows), a.group, lo + i, W) <= ti;
+        const bool in = i < cnt && kv4_first_tile(start(64 * (lo + i)), a.group, 64 * (lo + i), W) <= ti;
         const uint64_t m = __ballot(in);
         const int last = m ? 63 - __clzll(m) : 0;
         lo += last * step;
         cnt = min(step, cnt - last * step);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    t.b = lo;
-    t.r0 = a.row_start[lo];
-    const int r1 = a.row_start[lo + 1];
-    t.len = a.lengths[lo];
-    if (t.r0 < 0 || r1 > a.rows || r1 <= t.r0 || t.len < 0 || t.len > INT32_MAX - KV4_PAGE) return false;
-    t.n = r1 - t.r0;
+    lo = __builtin_amdgcn_readfirstlane(lo) * 64;
+    // what a lane's sequence is comes with the same wait as its rows
+    const int b = min(lo + lane, a.n_seqs), r0 = a.row_start[b], r1 = a.row_start[min(b + 1, a.n_seqs)];
+    const int len = a.lengths[min(b, a.n_seqs - 1)];
+    const int s0 = min(max(r0, 0), a.rows), s1 = min(max(r1, 0), a.rows);
+    const int tiles = max(((s1 - s0) * a.group + W - 1) / W, 0);
+    int end = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int below = __shfl_up(end, d);
+        if (lane >= d) end += below;
+    }
+    const int64_t rel = ti - kv4_first_tile(__builtin_amdgcn_readlane(s0, 0), a.group, lo, W);
+    const uint64_t m = __ballot(rel >= end - tiles && rel < end);
+    if (!m) return false;
+    const int at = __ffsll((unsigned long long)m) - 1;
+    t.b = lo + at;
+    t.r0 = __builtin_amdgcn_readlane(r0, at);
+    const int last = __builtin_amdgcn_readlane(r1, at);
+    t.len = __builtin_amdgcn_readlane(len, at);
+    if (t.r0 < 0 || last > a.rows || last <= t.r0 || t.len < 0 || t.len > INT32_MAX - KV4_PAGE) return false;
+    t.n = last - t.r0;
     t.ncols = t.n * a.group;
-    const int64_t rel = ti - kv4_first_tile(t.r0, a.group, lo, W);
-    if (rel < 0 || rel * W >= t.ncols) return false;
-    t.cb = (int)rel * W;
-    return true;
+    t.cb = (int)(rel - __builtin_amdgcn_readlane(end - tiles, at)) * W;
+    return t.cb < t.ncols;
 }
 
 // The last position that a column sees is len - n + row; minpos and maxpos are
@@ -569,6 +638,13 @@ __device__ __forceinline__ void tile_pages(const Kv4Attn &a, const AttnTile &t, 
 __device__ __forceinline__ int tile_parts(int pages, int chunk, int splits)
 {
     return max(1, min((pages + chunk - 1) / chunk, splits));
+}
+
+// Whether a position sees any key of a page.
+__device__ __forceinline__ bool sees(int pos, int window, int page)
+{
+    const int first = page * KV4_PAGE;
+    return pos >= first && (!window || pos - window < first + KV4_PAGE - 1);
 }
 
 // One page's block as a wave holds it: lane l = (r, kg) = (l % 16, l / 16) has
@@ -672,15 +748,42 @@ __device__ __forceinline__ float load_query(Query<T, D> &q, const T *p, bool val
     return unit;
 }
 
-// Running state of 16 columns in a wave: lane (m, kg) holds column m's maximum
+// Column cc of a tile: its query, its position (-1: there is no such column)
+// and the factor from products to log2 units.
+template <class T, int D>
+__device__ __forceinline__ float load_column(Query<T, D> &q, const Kv4Attn &a, const AttnTile &t, int hk, int cc, int kg, int &pos)
+{
+    const int row = cc / a.group;
+    const bool valid = cc < t.ncols;
+    pos = valid ? t.len - t.n + row : -1;
+    const T *qp = (const T *)a.q + (t.r0 + row) * a.q_stride + (hk * a.group + cc % a.group) * D + kg * (D / 4);
+    float unit = load_query<T, D>(q, qp, valid, a.vec) * (a.scale * 1.44269504088896341f);
+    if (a.scale < 0.0f) {            // the running maximum is taken before the factor
+        unit = -unit;
+#pragma unroll
+        for (int i = 0; i < Query<T, D>::PARTS; i++)
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) q.f[i][j] = -q.f[i][j];
+    }
+    return fmaxf(unit, 1.2e-38f);    // 0 * -inf would be NaN
+}
+
+// Running state of 16 columns in a wave: lane (m, kg) holds column m's reference
 // (in units of log2), its own share of the sum, and rows D/16 (4 kg + e) + i of
-// the output as o[i][e].  Probabilities are kept times 2^14, where f16 holds
-// the small ones too; sums and outputs carry the factor until they are divided.
+// the output as o[i][e].  The reference is a score that was the largest when
+// it was taken.  A probability is kept times 2^TOP over the reference's, where
+// f16 holds the small ones too, and the reference moves (sum and output are
+// scaled) only when one would pass 2^15: most pages neither exchange maxima
+// between lanes nor touch the output.  16-bit rows, whose probabilities are
+// rounded to f16's 11 bits anyway, leave more room for that than f32 rows.
+// Sums and outputs carry the factor until they are divided.
 template <int D>
 struct Running {
     float m = -INFINITY, l = 0.0f;
     f32x4 o[D / 16] = {};
 };
+template <class T>
+constexpr float TOP = std::is_same<T, float>::value ? 14.0f : 9.0f;
 
 // Scores of one page's 64 keys: lane (m, kg) gets column m's of keys 16 kg + 4 i
 // + t as x[t][i].
@@ -704,10 +807,8 @@ __device__ __forceinline__ void page_scores(f32x4 (&x)[4], const Unpack &un, con
     }
 }
 
-// The page at an edge: keys that a column does not see, and values past the
-// sequence's end, which may hold anything, count as zero (0 * NaN is not 0).
-template <int D>
-__device__ __forceinline__ void page_edge(f32x4 (&x)[4], PageV<D> &g, int key0, int pos, int window, int len, int kg)
+// Keys that a column does not see.
+__device__ __forceinline__ void mask_scores(f32x4 (&x)[4], int key0, int pos, int window, int kg)
 {
     const int first = key0 + 16 * kg;
     const int low = window ? pos - window : -1;
@@ -718,75 +819,120 @@ __device__ __forceinline__ void page_edge(f32x4 (&x)[4], PageV<D> &g, int key0, 
             const int key = first + 4 * i + t;
             if (key > pos || key <= low) x[t][i] = -INFINITY;
         }
+}
+
+// Scales of the values at positions first, first + 1, .. (two to a word), zero
+// past the sequence's end: what is there may be anything, and 0 * NaN is not 0.
+template <int N>
+__device__ __forceinline__ void mask_values(uint32_t (&scales)[N], int first, int len)
+{
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < N; i++) {
         const int left = len - (first + 2 * i);
-        g.s[i] = left <= 0 ? 0u : left == 1 ? g.s[i] & 0xFFFFu : g.s[i];
+        scales[i] = left <= 0 ? 0u : left == 1 ? scales[i] & 0xFFFFu : scales[i];
     }
 }
 
-// The running softmax, and P V on the lanes that hold the scores: nothing goes
-// from lane to lane but the maximum.
-template <class T, int D>
-__device__ __forceinline__ void page_values(Running<D> &s, const Unpack &un, f32x4 (&x)[4], const PageV<D> &g, float unit)
+// The running softmax over a page's scores, NC sets of 16 columns: probabilities
+// of keys 16 kg + 4 i + t at 4 i + t, in f16 pairs, of two parts for f32 rows.
+template <class T, int D, int NC>
+__device__ __forceinline__ void page_softmax(Running<D> (&s)[NC], f32x4 (&x)[NC][4], const float (&unit)[NC],
+                                             half8 (&p8)[NC][Query<T, D>::PARTS][2])
 {
-    constexpr int PARTS = Query<T, D>::PARTS;
-    float top = -INFINITY;
+    float off[NC], top[NC];
+    bool move = false;
 #pragma unroll
-    for (int t = 0; t < 4; t++) top = fmaxf(top, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
-    top = max_xor32(max_xor16(top)) * unit;
-    const float m = fmaxf(s.m, top);
-    if (__any(m > s.m)) {
-        const float f = m > s.m ? __builtin_amdgcn_exp2f(s.m - m) : 1.0f;   // exp2(-inf) = 0 at the first page
-        s.l *= f;
+    for (int c = 0; c < NC; c++) {
+        off[c] = s[c].m == -INFINITY ? 0.0f : TOP<T> - s[c].m;
+        top[c] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) s.o[i] *= f;
-        s.m = m;
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[c][t][i] = fmaf(x[c][t][i], unit[c], off[c]);      // the exponent
+                top[c] = fmaxf(top[c], x[c][t][i]);
+            }
+        move |= top[c] > (s[c].m == -INFINITY ? -INFINITY : 15.0f);
     }
-    const float off = m == -INFINITY ? 0.0f : 14.0f - m;
-    float p[16];                     // key 16 kg + 4 i + t at 4 i + t
+    if (__any(move)) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int c = 0; c < NC; c++) {
+            const float m = fmaxf(s[c].m, max_xor32(max_xor16(top[c])) - off[c]);
+            const float f = m > s[c].m ? __builtin_amdgcn_exp2f(s[c].m - m) : 1.0f;   // exp2(-inf) = 0 at the first page
+            const float by = m == -INFINITY ? 0.0f : TOP<T> - m - off[c];
+            s[c].l *= f;
+            s[c].m = m;
 #pragma unroll
-        for (int t = 0; t < 4; t++) p[4 * i + t] = __builtin_amdgcn_exp2f(fmaf(x[t][i], unit, off));
-    float sum = 0.0f;
+            for (int i = 0; i < D / 16; i++) s[c].o[i] *= f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) sum += p[i];
-    s.l += sum;
+            for (int t = 0; t < 4; t++) x[c][t] += by;
+        }
+    }
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        uint32_t ph[4], pl[4];
+    for (int c = 0; c < NC; c++) {
+        float p[16], sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 4; n++) split_f16_pair<true>(p[8 * u + 2 * n], p[8 * u + 2 * n + 1], ph[n], pl[n]);
-        const half8 p8 = as_half8(ph[0], ph[1], ph[2], ph[3]);
+        for (int i = 0; i < 16; i++) {
+            p[i] = __builtin_amdgcn_exp2f(x[c][i % 4][i / 4]);
+            sum += p[i];
+        }
+        s[c].l += sum;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float p0 = p[8 * u + 2 * n], p1 = p[8 * u + 2 * n + 1];
+                if constexpr (Query<T, D>::PARTS == 2)
+                    split_f16_pair<true>(p0, p1, ph[n], pl[n]);
+                else
+                    ph[n] = as_u(h16x2{(_Float16)p0, (_Float16)p1});
+            }
+            p8[c][0][u] = as_half8(ph[0], ph[1], ph[2], ph[3]);
+            if constexpr (Query<T, D>::PARTS == 2) p8[c][1][u] = as_half8(pl[0], pl[1], pl[2], pl[3]);
+        }
+    }
+}
+
+// o += V p over 32 keys, the small part first.
+template <int PARTS>
+__device__ __forceinline__ void add_values(f32x4 &o, half8 v8, const half8 (&p8)[PARTS][2], int u)
+{
+    if constexpr (PARTS == 2) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p8[1][u], o, 0, 0, 0);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p8[0][u], o, 0, 0, 0);
+}
+
+// P V on the lanes that hold the scores: nothing goes from lane to lane but
+// the maximum.
+template <class T, int D>
+__device__ __forceinline__ void page_values(Running<D> (&s)[1], const Unpack &un, f32x4 (&x)[1][4], const PageV<D> &g,
+                                            const float (&unit)[1])
+{
+    half8 p8[1][Query<T, D>::PARTS][2];
+    page_softmax<T, D, 1>(s, x, unit, p8);
+#pragma unroll
+    for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int c = 0; c < D / 64; c++) {       // units of four columns
             uint32_t a[4][4];
 #pragma unroll
             for (int h = 0; h < 4; h++) unpack8(un, g.v[2 * u + h / 2][2 * c + h % 2], as_h2(g.s[4 * u + h]), a[h]);
 #pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const half8 v8 = as_half8(a[0][n], a[1][n], a[2][n], a[3][n]);
-                f32x4 &o = s.o[4 * c + n];
-                if constexpr (PARTS == 2)
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, as_half8(pl[0], pl[1], pl[2], pl[3]), o, 0, 0, 0);
-                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p8, o, 0, 0, 0);
-            }
+            for (int n = 0; n < 4; n++) add_values(s[0].o[4 * c + n], as_half8(a[0][n], a[1][n], a[2][n], a[3][n]), p8[0], u);
         }
-    }
 }
 
 // Attention of 16 columns of one kv head over a share of the tile's pages, the
 // four waves taking them in turn and joining through LDS.
 template <class T, int D>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, 3)
 k_kv4_attn(Kv4Attn a)
 {
     constexpr int W = KV4_W, LD = D + 4;
     __shared__ float so[4][W][LD], sm[4][W], sl[4][W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kg = lane >> 4;
-    const int ti = blockIdx.x, sp = blockIdx.y, hk = blockIdx.z;
+    const int ti = blockIdx.x / a.cache.heads, hk = blockIdx.x % a.cache.heads, sp = blockIdx.y;
     AttnTile t;
     if (!find_tile(a, ti, W, t)) return;
     int minpos, maxpos, pg0, pages;
@@ -795,61 +941,52 @@ k_kv4_attn(Kv4Attn a)
     if (sp >= parts) return;
     const int pb = pg0 + sp * a.chunk, pe = sp == parts - 1 ? pg0 + pages : pb + a.chunk;
 
-    const int cc = t.cb + r, row = cc / a.group;
-    const bool valid = cc < t.ncols;
-    const int pos = valid ? t.len - t.n + row : -1;
     Query<T, D> q;
-    const T *qp = (const T *)a.q + (t.r0 + row) * a.q_stride + (hk * a.group + cc % a.group) * D + kg * (D / 4);
-    float unit = load_query<T, D>(q, qp, valid, a.vec) * (a.scale * 1.44269504088896341f);
-    if (a.scale < 0.0f) {            // the running maximum is taken before the factor
-        unit = -unit;
-#pragma unroll
-        for (int i = 0; i < Query<T, D>::PARTS; i++)
-#pragma unroll
-            for (int j = 0; j < D / 32; j++) q.f[i][j] = -q.f[i][j];
-    }
-
-    unit = fmaxf(unit, 1.2e-38f);    // 0 * -inf would be NaN
-    Running<D> s;
+    int pos;
+    const float unit[1] = {load_column<T, D>(q, a, t, hk, t.cb + r, kg, pos)};
+    Running<D> run[1];
     bool poisoned = pos >= (int64_t)a.max_pages * KV4_PAGE;   // sees a page that the table has no column for
     const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
     const Unpack un;
     const LaneAt<D> at(r, kg);
     const int n = (pe - pb - wave + 3) / 4;      // this wave's pages: pb + wave + 4 i
-    int i = -1, page = 0, ids = 0;               // ids: of 64 of them, one a lane
+    int ids = 0;                                 // of 64 of them, one a lane
     const uint8_t *blk = nullptr;
-    const auto next = [&] {
-        while (++i < n) {
-            page = pb + wave + 4 * i;
-            if ((i & 63) == 0) ids = page + 4 * lane < pe ? table[page + 4 * lane] : -1;
-            const int id = __builtin_amdgcn_readlane(ids, i & 63);
-            if (id >= 0 && id < a.cache.n_pages) {
-                blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
-                return true;
-            }
-            const int first = page * KV4_PAGE;   // what sees this page is NaN
-            poisoned |= pos >= first && (!a.window || pos - a.window < first + KV4_PAGE - 1);
+    int held = 0;                                // positions whose values count
+    const auto find = [&](int i) {
+        const int page = pb + wave + 4 * i;
+        if ((i & 63) == 0) ids = page + 4 * lane < pe ? table[page + 4 * lane] : -1;
+        int id = __builtin_amdgcn_readlane(ids, i & 63);
+        held = t.len;
+        if (id < 0 || id >= a.cache.n_pages) {   // what sees this page is NaN, and for the others its values are zero
+            id = held = 0;
+            poisoned |= sees(pos, a.window, page);
         }
-        return false;
+        blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
     };
     // V is on its way while K is multiplied, the next page's K while V is
     PageK<D> gk;
-    bool more = next();
-    if (more) load_page(gk, blk, at);
-    while (more) {
+    if (n > 0) {
+        find(0);
+        load_page(gk, blk, at);
+    }
+    for (int i = 0; i < n; i++) {
         PageV<D> gv;
         load_page(gv, blk, at);
-        const int key0 = page * KV4_PAGE;
-        f32x4 x[4];
+        const int key0 = (pb + wave + 4 * i) * KV4_PAGE, count = held;
+        f32x4 x[1][4];
         __builtin_amdgcn_sched_barrier(0);
-        page_scores<T, D>(x, un, gk, q);
+        page_scores<T, D>(x[0], un, gk, q);
         __builtin_amdgcn_sched_barrier(0);
-        more = next();
-        if (more) load_page(gk, blk, at);
-        if (key0 + KV4_PAGE - 1 > minpos || (a.window && key0 <= maxpos - a.window))
-            page_edge<D>(x, gv, key0, pos, a.window, t.len, kg);
-        page_values<T, D>(s, un, x, gv, unit);
+        if (i + 1 < n) {
+            find(i + 1);
+            load_page(gk, blk, at);
+        }
+        if (key0 + KV4_PAGE - 1 > minpos || (a.window && key0 <= maxpos - a.window)) mask_scores(x[0], key0, pos, a.window, kg);
+        if (key0 + KV4_PAGE > count) mask_values(gv.s, key0 + 16 * kg, count);
+        page_values<T, D>(run, un, x, gv, unit);
     }
+    Running<D> &s = run[0];
     s.l = add_xor32(add_xor16(s.l));
     if (poisoned) s.l = __builtin_nanf("");
     if (kg == 0) sm[wave][r] = s.m, sl[wave][r] = s.l;
@@ -876,7 +1013,7 @@ k_kv4_attn(Kv4Attn a)
             l += sm[w][c] == -INFINITY ? 0.0f * sl[w][c] : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - Mc);
         }
         if (parts > 1) {
-            if (d == 0) a.part[pi * 32 + c] = Mc, a.part[pi * 32 + 16 + c] = l;
+            if (d == 0) a.part[pi * 2 * W + c] = Mc, a.part[(pi * 2 + 1) * W + c] = l;
             *(f32x4 *)(a.part + a.part_rows + (pi * W + c) * D + d) = o;
         } else {
             // a column that saw nothing has l = 0
@@ -886,28 +1023,214 @@ k_kv4_attn(Kv4Attn a)
     }
 }
 
+// A page of a prompt's tile as a thread loads it: of eight shares, one for each
+// of the four K tiles (rows 4r + share) and of the four V blocks (positions 16
+// kg + 4 share .. + 3), each wave takes two or one, so that each code of the
+// page is unpacked once for the whole workgroup.
+template <int D>
+struct PageShare {
+    uint32_t k[D / 32], v[D / 32], vs[2];
+    uint16_t ks;
+    int held;                        // positions whose values count
+};
+
+constexpr int DS_STAYS = 0x47F;      // sched_barrier: all but LDS instructions may pass
+
+// Attention of W = 128 columns of one kv head, NC sets of 16 a wave: the prompt
+// path.  A page is unpacked to f16 once and laid in LDS in the order in which
+// the matrix instructions read it (1 KiB a fragment, each lane its 16 bytes),
+// one page ahead of the products.  Two sets a wave halve the LDS reads of a
+// product; f32 rows, whose queries and probabilities have two parts, do that
+// with one set, and take eight waves instead of four.
+template <class T, int D, int NC>
+__global__ void __launch_bounds__(KV4_WIDE / NC * 4, 2)
+k_kv4_attn_rows(Kv4Attn a)
+{
+    constexpr int W = KV4_WIDE, WAVES = W / (16 * NC), KF = D / 8, VF = D / 8;   // fragments of a page: 4 x D/32 and 2 x D/16
+    __shared__ u32x4 lk[2][KF][64], lv[2][VF][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, kg = lane >> 4;
+    const bool takes_k = WAVES == 4 || wave < 4, takes_v = WAVES == 4 || wave >= 4;
+    const int share = wave & 3;
+    // the last tiles of a sequence see the most: they go first
+    const int bx = gridDim.x - 1 - blockIdx.x, ti = bx / a.cache.heads, hk = bx % a.cache.heads, sp = blockIdx.y;
+    AttnTile t;
+    if (!find_tile(a, ti, W, t)) return;
+    int minpos, maxpos, pg0, pages;
+    tile_pages(a, t, W, minpos, maxpos, pg0, pages);
+    const int parts = tile_parts(pages, a.chunk, a.splits);
+    if (sp >= parts) return;
+    const int pb = pg0 + sp * a.chunk, pe = sp == parts - 1 ? pg0 + pages : pb + a.chunk;
+
+    constexpr int PARTS = Query<T, D>::PARTS;
+    Query<T, D> q[NC];
+    int pos[NC], low[NC], high[NC];  // low, high: the first and last position of 16 columns
+    float unit[NC];
+    Running<D> s[NC];
+    bool poisoned[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int first = t.cb + (wave * NC + c) * 16;
+        unit[c] = load_column<T, D>(q[c], a, t, hk, first + r, kg, pos[c]);
+        low[c] = t.len - t.n + first / a.group;
+        high[c] = first < t.ncols ? t.len - t.n + min(first + 15, t.ncols - 1) / a.group : -1;
+        poisoned[c] = pos[c] >= (int64_t)a.max_pages * KV4_PAGE;
+    }
+    const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
+    const Unpack un;
+    const LaneAt<D> at(r, kg);
+    int ids = 0;                                 // of 64 pages, one a lane
+    const auto fetch = [&](PageShare<D> &g, int page) {
+        const int i = (page - pb) & 63;
+        if (i == 0) ids = page + lane < pe ? table[page + lane] : -1;
+        int id = __builtin_amdgcn_readlane(ids, i);
+        g.held = t.len;
+        if (id < 0 || id >= a.cache.n_pages) {   // what sees this page is NaN, and for the others its values are zero
+            id = 0;
+            g.held = 0;
+#pragma unroll
+            for (int c = 0; c < NC; c++) poisoned[c] |= sees(pos[c], a.window, page);
+        }
+        const uint8_t *blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
+        if (takes_k) {
+            load_words<D>(g.k, blk + share * (kv4_k_at(D, 1) - kv4_k_at(D, 0)) + at.k);
+            g.ks = *(const uint16_t *)(blk + share * 2 + at.ks);
+        }
+        if (takes_v) {
+            load_words<D>(g.v, blk + share * (kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0)) + at.v);
+            const uint2 vs = *(const uint2 *)(blk + share * 8 + at.vs);
+            g.vs[0] = vs.x, g.vs[1] = vs.y;
+        }
+    };
+    const auto stage = [&](PageShare<D> &g, int key0, int buf) {
+        if (takes_k) {
+            const h16x2 ks = as_h2((uint32_t)g.ks | (uint32_t)g.ks << 16);
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) {
+                uint32_t k[4];
+                unpack8(un, g.k[j], ks, k);
+                lk[buf][share * (D / 32) + j][lane] = u32x4{k[0], k[1], k[2], k[3]};
+            }
+        }
+        if (takes_v) {
+            if (key0 + KV4_PAGE > g.held) mask_values(g.vs, key0 + 16 * kg + 4 * share, g.held);
+#pragma unroll
+            for (int c = 0; c < D / 64; c++) {
+                uint32_t v0[4], v1[4];
+                unpack8(un, g.v[2 * c], as_h2(g.vs[0]), v0);
+                unpack8(un, g.v[2 * c + 1], as_h2(g.vs[1]), v1);
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    *((uint2 *)&lv[buf][share / 2 * (D / 16) + 4 * c + n][lane] + share % 2) = make_uint2(v0[n], v1[n]);
+            }
+        }
+    };
+
+    PageShare<D> g;
+    if (pb < pe) {
+        fetch(g, pb);
+        stage(g, pb * KV4_PAGE, 0);
+    }
+    __syncthreads();
+    for (int page = pb; page < pe; page++) {
+        const int key0 = page * KV4_PAGE, buf = (page - pb) & 1;
+        if (page + 1 < pe) fetch(g, page + 1);
+        // fragments are read from LDS in pairs, two pairs ahead of the products; the
+        // reads stay where they are written (otherwise each is waited for by itself)
+        f32x4 x[NC][4];
+        half8 f[3][2];
+        const auto read = [&](half8 (&to)[2], const u32x4 (*from)[64], int n) {
+            to[0] = __builtin_bit_cast(half8, from[2 * n][lane]);
+            to[1] = __builtin_bit_cast(half8, from[2 * n + 1][lane]);
+        };
+        read(f[0], lk[buf], 0);
+        read(f[1], lk[buf], 1);
+#pragma unroll
+        for (int n = 0; n < KF / 2; n++) {
+            if (n < KF / 2 - 2) read(f[(n + 2) % 3], lk[buf], n + 2);
+            __builtin_amdgcn_sched_barrier(DS_STAYS);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = (2 * n + h) / (D / 32), j = (2 * n + h) % (D / 32);    // K tile and step
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+                        x[c][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            f[n % 3][h], q[c].f[part][j], j == 0 && part == PARTS - 1 ? f32x4{0, 0, 0, 0} : x[c][k], 0, 0, 0);
+            }
+        }
+        read(f[0], lv[buf], 0);
+        read(f[1], lv[buf], 1);
+        half8 p8[NC][PARTS][2];
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            if (key0 + KV4_PAGE - 1 > low[c] || (a.window && key0 <= high[c] - a.window))
+                mask_scores(x[c], key0, pos[c], a.window, kg);
+        }
+        page_softmax<T, D, NC>(s, x, unit, p8);
+#pragma unroll
+        for (int n = 0; n < VF / 2; n++) {
+            if (n < VF / 2 - 2) read(f[(n + 2) % 3], lv[buf], n + 2);
+            __builtin_amdgcn_sched_barrier(DS_STAYS);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    add_values(s[c].o[(2 * n + h) % (D / 16)], f[n % 3][h], p8[c], (2 * n + h) / (D / 16));
+        }
+        if (page + 1 < pe) stage(g, key0 + KV4_PAGE, buf ^ 1);
+        __syncthreads();
+    }
+    const int64_t pi = ((int64_t)ti * a.cache.heads + hk) * a.splits + sp;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int cw = (wave * NC + c) * 16 + r, col = t.cb + cw;
+        float l = add_xor32(add_xor16(s[c].l));
+        if (poisoned[c]) l = __builtin_nanf("");
+        if (col >= t.ncols) continue;
+        if (parts > 1) {
+            if (kg == 0) a.part[pi * 2 * W + cw] = s[c].m, a.part[(pi * 2 + 1) * W + cw] = l;
+            float *o = a.part + a.part_rows + (pi * W + cw) * D + D / 4 * kg;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 4)
+                    *(f32x4 *)(o + D / 16 * e + i) = f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]};
+        } else {
+            T *o = (T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + D / 4 * kg;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a column that saw nothing has o = 0
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 4)
+                    store4(o + D / 16 * e + i, f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]} * inv, a.vec);
+        }
+    }
+}
+
 // The parts of a tile's columns joined, one column at a time: weights 2^(m - M),
 // then the rows' weighted sum, 256 / (D / 4) of them at once.
-template <class T, int D>
+template <class T, int D, int W>
 __global__ void __launch_bounds__(256)
 k_kv4_attn_join(Kv4Attn a)
 {
     constexpr int L = D / 4, ROWS = 256 / L;
     __shared__ float w[64];
     __shared__ f32x4 so[ROWS][L];
-    const int ti = blockIdx.x, hk = blockIdx.z, lane = threadIdx.x & 63;
+    const int ti = blockIdx.x / a.cache.heads, hk = blockIdx.x % a.cache.heads, lane = threadIdx.x & 63;
     AttnTile t;
-    if (!find_tile(a, ti, KV4_W, t)) return;
+    if (!find_tile(a, ti, W, t)) return;
     int minpos, maxpos, pg0, pages;
-    tile_pages(a, t, KV4_W, minpos, maxpos, pg0, pages);
+    tile_pages(a, t, W, minpos, maxpos, pg0, pages);
     const int parts = tile_parts(pages, a.chunk, a.splits);
     if (parts == 1) return;
     const int64_t p0 = ((int64_t)ti * a.cache.heads + hk) * a.splits;
     const int i = threadIdx.x % L, g = threadIdx.x / L;
-    for (int c = blockIdx.y; c < min(KV4_W, t.ncols - t.cb); c += gridDim.y) {
+    for (int c = blockIdx.y; c < min(W, t.ncols - t.cb); c += gridDim.y) {
         const int col = t.cb + c;
         float m = -INFINITY, l = 0.0f;
-        if (lane < parts) m = a.part[(p0 + lane) * 32 + c], l = a.part[(p0 + lane) * 32 + 16 + c];
+        if (lane < parts) m = a.part[(p0 + lane) * 2 * W + c], l = a.part[((p0 + lane) * 2 + 1) * W + c];
         const float M = wave_max_dpp(m);
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
         const float sum = wave_sum_dpp(l * f);
@@ -916,7 +1239,7 @@ k_kv4_attn_join(Kv4Attn a)
         __syncthreads();
         f32x4 o = {0, 0, 0, 0};
         for (int s = g; s < parts; s += ROWS)
-            o += *(const f32x4 *)(a.part + a.part_rows + ((p0 + s) * KV4_W + c) * D + 4 * i) * w[s];
+            o += *(const f32x4 *)(a.part + a.part_rows + ((p0 + s) * W + c) * D + 4 * i) * w[s];
         so[g][i] = o;
         __syncthreads();
         if (g) continue;
@@ -930,34 +1253,72 @@ k_kv4_attn_join(Kv4Attn a)
 // Tiles there can be: the number after the last sequence's last.
 static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return kv4_first_tile(rows, group, n_seqs, W); }
 
-// Pages that a workgroup takes, and the most workgroups of a tile.
-void kv4_attn_split(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window, int *chunk, int *splits)
+// How a call is cut: columns of a tile, pages of a workgroup, the most
+// workgroups of a tile.
+//
+// The wide tiles unpack a page once for 128 columns, but a workgroup's way
+// through its pages takes longer (1.9 us a page, 16 columns 0.9), so they pay
+// where there are many: 32 sequences of 2048 positions, bf16, take with 16
+// columns / wide 51 / 63 us for 32 rows each, 94 / 67 for 64, 179 / 96 for 128,
+// but 8 sequences 51 / 78 for 128 rows; of 400 positions, 64 sequences 22 / 27
+// for 16 rows, 36 / 31 for 32, 64 / 39 for 64.
+//
+// Splitting a tile's pages costs a second kernel (5 us, and its launch), and
+// pays where workgroups are few: 16 sequences of 16000 positions in 1024 parts 45
+// us, in 256 81; 64 of 1365 to 4096, 512 workgroups, 53 whole and 61 in two.  So
+// up to 16 pages, four for each of a workgroup's waves, stay whole (one sequence
+// of 700 11 us, in two 15), and so do shorter ones than 64 pages (wide: 128) where
+// the card is full without; longer ones are split for the sake of the shorter
+// ones beside them.
+Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
 {
-    const int64_t items = attn_tiles(rows, n_seqs, group, KV4_W) * kv_heads;
+    Kv4Cut c{};
+    const int64_t cols = n_seqs ? rows * group / n_seqs : 0;     // of an average sequence
+    const bool wide = cols >= 48 && rows * group * kv_heads >= 24576;
+    c.width = wide ? KV4_WIDE : KV4_W;
+    const int64_t items = std::max<int64_t>(attn_tiles(rows, n_seqs, group, c.width) * kv_heads, 1);
     int64_t pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
-    if (window) pages = std::min<int64_t>(pages, (window + KV4_W - 2) / KV4_PAGE + 2);
-    int64_t per = std::max<int64_t>(items * pages / 1024, (pages + 63) / 64);
-    per = std::max<int64_t>((per + 3) / 4 * 4, 4);
-    *chunk = (int)std::min<int64_t>(per, INT32_MAX / KV4_PAGE);
-    *splits = (int)std::max<int64_t>(1, (pages + per - 1) / per);
+    if (window) pages = std::min<int64_t>(pages, ((int64_t)window + c.width - 2) / KV4_PAGE + 2);
+    int64_t per;
+    if (wide)
+        per = items >= 256 ? 128 : std::max<int64_t>(items * pages / 512, 8);
+    else
+        per = items >= 512 ? 64 : pages <= 16 ? 16 : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);
+    per = std::max<int64_t>(per, (pages + 63) / 64);
+    c.chunk = (int)std::min<int64_t>(per, INT32_MAX / KV4_PAGE);
+    c.splits = (int)std::max<int64_t>(1, (pages + per - 1) / per);
+    c.parts = c.splits > 1 && rows && n_seqs ? items * c.splits : 0;
+    return c;
 }
 
+// The kv heads of a tile are neighbours in the grid: workgroups go round the
+// XCDs one by one, and so each XCD gets as much of a long sequence as of a
+// short one (64 sequences of 1365 to 4096 positions: 53 us, with the tiles as
+// neighbours 59).
 template <class T, int D>
-static hipError_t launch_attn(const Kv4Attn &a, hipStream_t s)
+static hipError_t launch_attn(const Kv4Attn &a, int width, hipStream_t s)
 {
-    const unsigned tiles = (unsigned)attn_tiles(a.rows, a.n_seqs, a.group, KV4_W);
-    hipLaunchKernelGGL((k_kv4_attn<T, D>), dim3(tiles, a.splits, a.cache.heads), dim3(256), 0, s, a);
+    const unsigned tiles = (unsigned)attn_tiles(a.rows, a.n_seqs, a.group, width);
+    const bool wide = width == KV4_WIDE;
+    constexpr int NC = 2;
+    if (wide)
+        hipLaunchKernelGGL((k_kv4_attn_rows<T, D, NC>), dim3(tiles * a.cache.heads, a.splits), dim3(KV4_WIDE / NC * 4), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_kv4_attn<T, D>), dim3(tiles * a.cache.heads, a.splits), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     // a workgroup a column of an average sequence's tile
-    const int64_t cols = std::min<int64_t>(KV4_W, ((int64_t)a.rows * a.group + a.n_seqs - 1) / a.n_seqs);
-    hipLaunchKernelGGL((k_kv4_attn_join<T, D>), dim3(tiles, (unsigned)cols, a.cache.heads), dim3(256), 0, s, a);
+    const unsigned cols = (unsigned)std::min<int64_t>(width, ((int64_t)a.rows * a.group + a.n_seqs - 1) / a.n_seqs);
+    if (wide)
+        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_WIDE>), dim3(tiles * a.cache.heads, cols), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_W>), dim3(tiles * a.cache.heads, cols), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
-hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, hipStream_t s)
+hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, int width, hipStream_t s)
 {
-    KV4_TYPED(dtype, D, (launch_attn<T, HD>(a, s)));
+    KV4_TYPED(dtype, D, (launch_attn<T, HD>(a, width, s)));
 }
 
 }  // namespace qtts

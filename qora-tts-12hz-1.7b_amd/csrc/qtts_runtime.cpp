@@ -2080,8 +2080,9 @@ static int check_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a)
     if (a->rows < 0 || a->n_seqs < 0 || a->n_heads < 1 || a->n_heads % a->cache->n_kv_heads)
         return fail(c, QTTS_ERR_INVALID, "%lld rows, %d sequences, %d / %d heads", (long long)a->rows, a->n_seqs, a->n_heads,
                     a->cache->n_kv_heads);
-    if (a->rows > (1 << 27) / (int64_t)a->n_heads || a->n_seqs > (1 << 22))
-        return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 rows x heads and 2^22 sequences a call");
+    // keeps the grid's workgroups x 256 threads below 2^32
+    if (a->rows > (1 << 27) / (int64_t)a->n_heads || a->n_seqs > (1 << 22) / a->cache->n_kv_heads)
+        return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 rows x heads and 2^22 sequences x kv heads a call");
     RCHK(check_rows(c, "q", a->q, a->rows, a->n_heads, D, a->q_stride, a->dtype));
     RCHK(check_rows(c, "out", a->out, a->rows, a->n_heads, D, a->out_stride, a->dtype));
     if (a->max_pages < 1 || a->table_stride < a->max_pages || a->max_pages > INT32_MAX / KV4_PAGE - 2 || a->table_stride > INT32_MAX)
@@ -2100,25 +2101,18 @@ static int check_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a)
     return QTTS_OK;
 }
 
-// How a call's pages are split, and the parts whose results the workspace holds
-// (0: nothing is split).
-struct AttnSplit { int chunk, splits; int64_t parts; };
-static AttnSplit attention_split(const qtts_kv4_attention_args *a)
+static Kv4Cut attention_cut(const qtts_kv4_attention_args *a)
 {
-    const int group = a->n_heads / a->cache->n_kv_heads;
-    AttnSplit s{};
-    kv4_attn_split(a->rows, a->n_seqs, group, a->cache->n_kv_heads, a->max_len, a->window, &s.chunk, &s.splits);
-    if (s.splits > 1 && a->rows && a->n_seqs)
-        s.parts = kv4_first_tile(a->rows, group, a->n_seqs, KV4_W) * a->cache->n_kv_heads * s.splits;
-    return s;
+    return kv4_attn_cut(a->rows, a->n_seqs, a->n_heads / a->cache->n_kv_heads, a->cache->n_kv_heads, a->max_len, a->window);
 }
-static int64_t parts_bytes(const qtts_kv4_attention_args *a, int64_t parts) { return parts * (32 + KV4_W * a->cache->head_dim) * 4; }
+// Bytes of a call's partial results: maxima and sums, then rows.
+static int64_t parts_bytes(const Kv4Cut &c, int head_dim) { return c.parts * c.width * (2 + head_dim) * 4; }
 
 extern "C" int qtts_kv4_attention_workspace(const qtts_kv4_attention_args *a, int64_t *bytes)
 {
     if (!a || !bytes) return QTTS_ERR_INVALID;
     RCHK(check_kv4_attention(nullptr, a));
-    *bytes = parts_bytes(a, attention_split(a).parts);
+    *bytes = parts_bytes(attention_cut(a), a->cache->head_dim);
     return QTTS_OK;
 }
 
@@ -2126,8 +2120,8 @@ extern "C" int qtts_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a,
 {
     if (!a || (!c && !(flags & QTTS_CHECK_ONLY))) return QTTS_ERR_INVALID;
     RCHK(check_kv4_attention(c, a));
-    const AttnSplit split = attention_split(a);
-    const int64_t need = parts_bytes(a, split.parts);
+    const Kv4Cut cut = attention_cut(a);
+    const int64_t need = parts_bytes(cut, a->cache->head_dim);
     if (need > a->workspace_bytes || (need && !a->workspace) || (need && !kv4_aligned(a->workspace, 16)))
         return fail(c, QTTS_ERR_CAPACITY, "workspace of %lld bytes, 16-byte aligned, needed; %lld given", (long long)need,
                     (long long)a->workspace_bytes);
@@ -2144,11 +2138,11 @@ extern "C" int qtts_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a,
     k.row_start = a->row_start, k.lengths = a->lengths, k.table = a->table, k.table_stride = a->table_stride;
     k.part = (float *)a->workspace;
     k.rows = (int32_t)a->rows, k.n_seqs = a->n_seqs, k.max_pages = a->max_pages, k.group = a->n_heads / a->cache->n_kv_heads;
-    k.window = a->window, k.chunk = split.chunk, k.splits = split.splits, k.scale = a->scale;
-    k.part_rows = 32 * split.parts;
+    k.window = a->window, k.chunk = cut.chunk, k.splits = cut.splits, k.scale = a->scale;
+    k.part_rows = 2 * cut.parts * cut.width;
     k.vec = moves4(a->q, a->q_stride, a->dtype) && moves4(a->out, a->out_stride, a->dtype);
     DeviceGuard guard(c->device);
-    return kv4_done(c, enqueue_kv4_attn(k, a->dtype, (int)D, (hipStream_t)stream));
+    return kv4_done(c, enqueue_kv4_attn(k, a->dtype, (int)D, cut.width, (hipStream_t)stream));
 }
 
 // ---------------------------------------------------------------------------

@@ -136,15 +136,22 @@ def tables(self, cached, fresh, free_pages, table, rows, out=None):
         _load()
     device, i32 = self.device, _torch.int32
     n, free = cached.shape[0], free_pages.shape[0]
+    inputs = (_vector("cached", cached, n, i32, device), _vector("fresh", fresh, n, i32, device),
+              _vector("free_pages", free_pages, free, i32, device), free, table.data_ptr(), _table(table, n, device))
     if out is None:
         # one allocation for what is held in 32 bits
-        row_start, lengths, positions, status = cached.new_empty(2 * n + rows + 3).split_with_sizes([n + 1, n, rows, 2])
-        out = Kv4Step(row_start, lengths, positions, cached.new_empty(rows, dtype=_torch.int64), status)
-    a = _TABLES.pack(n, table.shape[1], _vector("cached", cached, n, i32, device), _vector("fresh", fresh, n, i32, device),
-                     _vector("free_pages", free_pages, free, i32, device), free, table.data_ptr(), _table(table, n, device),
-                     _vector("row_start", out.row_start, n + 1, i32, device), _vector("lengths", out.lengths, n, i32, device),
-                     _vector("positions", out.positions, rows, i32, device),
-                     _vector("slots", out.slots, rows, _torch.int64, device), rows, _vector("status", out.status, 2, i32, device))
+        both = cached.new_empty(2 * n + rows + 3)
+        slots = cached.new_empty(rows, dtype=_torch.int64)
+        at = both.data_ptr()
+        a = _TABLES.pack(n, table.shape[1], *inputs, at, at + 4 * n + 4, at + 8 * n + 4, slots.data_ptr(), rows,
+                         at + 8 * n + 4 * rows + 4)
+        row_start, lengths, positions, status = both.split_with_sizes([n + 1, n, rows, 2])
+        out = Kv4Step(row_start, lengths, positions, slots, status)
+    else:
+        a = _TABLES.pack(n, table.shape[1], *inputs, _vector("row_start", out.row_start, n + 1, i32, device),
+                         _vector("lengths", out.lengths, n, i32, device), _vector("positions", out.positions, rows, i32, device),
+                         _vector("slots", out.slots, rows, _torch.int64, device), rows,
+                         _vector("status", out.status, 2, i32, device))
     rc = self.lib.qtts_kv4_tables(self.h, a, _stream(device), 0)
     if rc:
         self._check(rc)
@@ -213,11 +220,12 @@ def gather(self, cache, slots, dtype):
         raise _elsewhere("the cache", cache.pages, device)
     n = slots.shape[0]
     at = _vector("slots", slots, n, _torch.int64, device)
-    K, V = slots.new_empty((2, n, cache.n_kv_heads, cache.head_dim), dtype=dtype).unbind()
-    rc = self.lib.qtts_kv4_gather(self.h, cache.address, at, n, _code("values", K), K.data_ptr(), V.data_ptr(), _stream(device), 0)
+    both = slots.new_empty((2, n, cache.n_kv_heads, cache.head_dim), dtype=dtype)
+    K = both.data_ptr()
+    rc = self.lib.qtts_kv4_gather(self.h, cache.address, at, n, _code("values", both), K, K + both.nbytes // 2, _stream(device), 0)
     if rc:
         self._check(rc)
-    return K, V
+    return both.unbind()
 
 
 def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, max_len=None, out=None):
@@ -246,8 +254,9 @@ def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, m
             _table(table, n, device), PAGE * columns if max_len is None else max_len, 1 / math.sqrt(dim) if scale is None else scale,
             window)
     a = _ATTENTION.pack(*head, 0, 0)
-    need = ctypes.c_int64()
-    self.lib.qtts_kv4_attention_workspace(a, ctypes.byref(need))     # what it refuses the call itself names
+    need = self._kv4_need
+    need.value = 0
+    self.lib.qtts_kv4_attention_workspace(a, self._kv4_need_at)      # what it refuses the call itself names
     if need.value:
         workspace = q.new_empty(need.value, dtype=_torch.uint8)
         a = _ATTENTION.pack(*head, workspace.data_ptr(), need.value)

@@ -329,13 +329,13 @@ def bound(kind, want, mag, big, lengths):
     product with V rounded to f16 (2^-11), or to two f16 (2^-22) for f32 rows; sums of
     weights and products in f32 run over at most pages + 96 additions in a row.
     Numerator and denominator each carry these: twice.  A weight is held as f16 at
-    2^14 times its share of the largest, so one below f16's smallest normal is off by
-    half of the subnormal step 2^-24: 2^-39 of the largest weight, for each key.  Then
-    the type's rounding."""
+    2^14 (f32 rows) or 2^9 times its share of a weight that is at most the largest, so
+    one below f16's smallest normal is off by half of the subnormal step 2^-24: 2^-39 or
+    2^-34 of the largest weight, for each key.  Then the type's rounding."""
     d = (128 * 2.0 ** -24 + (2.0 ** -22 if kind == "f32" else 0) + 4 * 2.0 ** -24) * big + 2.0 ** -21
     w = 2.0 ** -22 if kind == "f32" else 2.0 ** -11
     chain = (96 + max(lengths) / 64) * 2.0 ** -24
-    return 2 * (d[..., None] + w + chain) * mag[..., 0] + 2.0 ** -39 * mag[..., 1] + EPS[kind] * np.abs(want) * 1.001 + (6e-8 if kind == "f16" else 0)
+    return 2 * (d[..., None] + w + chain) * mag[..., 0] + 2.0 ** (-39 if kind == "f32" else -34) * mag[..., 1] + EPS[kind] * np.abs(want) * 1.001 + (6e-8 if kind == "f16" else 0)
 
 
 def off_rms(kind, big):

@@ -166,7 +166,8 @@ def test_workspace_grows_with_the_split_only():
     assert need(rows=1, n_seqs=1, max_len=10) == 0            # one page: nothing to split
     assert need(rows=1, n_seqs=1, max_len=16000) > 0
     assert need(rows=0, max_len=16000) == 0
-    assert need(rows=4096, n_seqs=4096, max_len=16000) == 0   # the sequences fill the card
+    assert need(rows=1, n_seqs=1, max_len=1024) == 0          # four pages for each wave
+    assert need(rows=4096, n_seqs=4096, max_len=4096) == 0    # the sequences fill the card
     assert need(rows=1, n_seqs=1, max_len=1 << 40) < 1 << 25
 
 
