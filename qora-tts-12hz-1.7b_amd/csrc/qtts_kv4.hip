@@ -261,7 +261,7 @@ __device__ __forceinline__ void norm_rope(Head<F> &x, bool norm, f32x4 ga, f32x4
 // order of values, so only two extremes that it makes equal have to be looked at
 // again, and the quotient (at most 16, off by 2^-22 of it from x, the reciprocal
 // and the product) only next to a half.  In f64 throughout, the quantisation of
-// 4001 rows of 16 heads took 22 us instead of TIME.
+// 4001 rows of 16 heads took 22.3 us instead of 18.7.
 template <class F>
 __device__ __forceinline__ uint32_t quantise(const F (&x)[4], uint16_t &scale)
 {
@@ -1023,10 +1023,9 @@ k_kv4_attn(Kv4Attn a)
     }
 }
 
-// A page of a prompt's tile as a thread loads it: of eight shares, one for each
-// of the four K tiles (rows 4r + share) and of the four V blocks (positions 16
-// kg + 4 share .. + 3), each wave takes two or one, so that each code of the
-// page is unpacked once for the whole workgroup.
+// A page of a prompt's tile as a thread loads it: each of four waves takes one
+// K tile (rows 4r + share) and one V block (positions 16 kg + 4 share .. + 3),
+// so that each code of the page is unpacked once for all four.
 template <int D>
 struct PageShare {
     uint32_t k[D / 32], v[D / 32], vs[2];
@@ -1036,22 +1035,35 @@ struct PageShare {
 
 constexpr int DS_STAYS = 0x47F;      // sched_barrier: all but LDS instructions may pass
 
-// Attention of W = 128 columns of one kv head, NC sets of 16 a wave: the prompt
-// path.  A page is unpacked to f16 once and laid in LDS in the order in which
-// the matrix instructions read it (1 KiB a fragment, each lane its 16 bytes),
-// one page ahead of the products.  Two sets a wave halve the LDS reads of a
-// product; f32 rows, whose queries and probabilities have two parts, do that
-// with one set, and take eight waves instead of four.
-template <class T, int D, int NC>
-__global__ void __launch_bounds__(KV4_WIDE / NC * 4, 2)
+// Attention of 128 columns of one kv head, two sets of 16 a wave: the prompt
+// path.  A page is unpacked to f16 once for four waves and laid in LDS in the
+// order in which the matrix instructions read it (1 KiB a fragment, each lane
+// its 16 bytes), one page ahead of the products; two sets a wave halve the LDS
+// reads of a product.  Matrix and other vector instructions of a SIMD hardly
+// overlap here (48 of 4.4 cycles and four of 16.6 take their sum, from one wave or
+// from two), so a page costs what its 425 vector instructions and 64 products a
+// wave add up to, 3000 cycles, and a fifth more for waits.
+//
+// HALVES 2, for no more tiles than CUs: eight waves, the second four taking every
+// other page, joined at the end.  The longest tile's way is half as long, and
+// each SIMD has two waves to take turns.  2048 positions, sequences of 64 rows, in
+// us with four waves / eight: 16 sequences (128 tiles) 65 / 51, 32 70 / 59, 64 104 /
+// 114, and four prompts of 500 to 1000 rows (376 tiles) 79 / 84: there two
+// workgroups of four share a CU more evenly.
+template <class T, int D, int HALVES>
+__global__ void __launch_bounds__(256 * HALVES, 2)
 k_kv4_attn_rows(Kv4Attn a)
 {
-    constexpr int W = KV4_WIDE, WAVES = W / (16 * NC), KF = D / 8, VF = D / 8;   // fragments of a page: 4 x D/32 and 2 x D/16
-    __shared__ u32x4 lk[2][KF][64], lv[2][VF][64];
+    constexpr int W = KV4_WIDE, NC = 2, KF = D / 8, VF = D / 8;  // fragments of a page: 4 x D/32 and 2 x D/16
+    constexpr int PARTS = Query<T, D>::PARTS, LD = D + 4;
+    static_assert(W == 4 * NC * 16, "four waves' columns");
+    // pages while they are multiplied: [half][buffer][K, then V fragments]; then the second half's result
+    __shared__ union {
+        u32x4 page[HALVES][2][KF + VF][64];
+        struct { float o[HALVES == 2 ? W : 1][LD], m[W], l[W]; } half;
+    } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, kg = lane >> 4;
-    const bool takes_k = WAVES == 4 || wave < 4, takes_v = WAVES == 4 || wave >= 4;
-    const int share = wave & 3;
+    const int r = lane & 15, kg = lane >> 4, share = wave & 3, half = HALVES == 2 ? wave >> 2 : 0;
     // the last tiles of a sequence see the most: they go first
     const int bx = gridDim.x - 1 - blockIdx.x, ti = bx / a.cache.heads, hk = bx % a.cache.heads, sp = blockIdx.y;
     AttnTile t;
@@ -1062,7 +1074,6 @@ k_kv4_attn_rows(Kv4Attn a)
     if (sp >= parts) return;
     const int pb = pg0 + sp * a.chunk, pe = sp == parts - 1 ? pg0 + pages : pb + a.chunk;
 
-    constexpr int PARTS = Query<T, D>::PARTS;
     Query<T, D> q[NC];
     int pos[NC], low[NC], high[NC];  // low, high: the first and last position of 16 columns
     float unit[NC];
@@ -1070,7 +1081,7 @@ k_kv4_attn_rows(Kv4Attn a)
     bool poisoned[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int first = t.cb + (wave * NC + c) * 16;
+        const int first = t.cb + (share * NC + c) * 16;
         unit[c] = load_column<T, D>(q[c], a, t, hk, first + r, kg, pos[c]);
         low[c] = t.len - t.n + first / a.group;
         high[c] = first < t.ncols ? t.len - t.n + min(first + 15, t.ncols - 1) / a.group : -1;
@@ -1079,62 +1090,59 @@ k_kv4_attn_rows(Kv4Attn a)
     const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
     const Unpack un;
     const LaneAt<D> at(r, kg);
-    int ids = 0;                                 // of 64 pages, one a lane
-    const auto fetch = [&](PageShare<D> &g, int page) {
-        const int i = (page - pb) & 63;
-        if (i == 0) ids = page + lane < pe ? table[page + lane] : -1;
-        int id = __builtin_amdgcn_readlane(ids, i);
+    int ids = 0;                     // of 64 pages, one a lane
+    const auto fetch = [&](PageShare<D> &g, int it) {
+        const int page = pb + HALVES * it + half;
+        if ((it & 63) == 0) ids = page + HALVES * lane < pe ? table[page + HALVES * lane] : -1;
+        int id = __builtin_amdgcn_readlane(ids, it & 63);
         g.held = t.len;
         if (id < 0 || id >= a.cache.n_pages) {   // what sees this page is NaN, and for the others its values are zero
             id = 0;
             g.held = 0;
 #pragma unroll
-            for (int c = 0; c < NC; c++) poisoned[c] |= sees(pos[c], a.window, page);
+            for (int c = 0; c < NC; c++) poisoned[c] |= page < pe && sees(pos[c], a.window, page);
         }
         const uint8_t *blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
-        if (takes_k) {
-            load_words<D>(g.k, blk + share * (kv4_k_at(D, 1) - kv4_k_at(D, 0)) + at.k);
-            g.ks = *(const uint16_t *)(blk + share * 2 + at.ks);
-        }
-        if (takes_v) {
-            load_words<D>(g.v, blk + share * (kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0)) + at.v);
-            const uint2 vs = *(const uint2 *)(blk + share * 8 + at.vs);
-            g.vs[0] = vs.x, g.vs[1] = vs.y;
-        }
+        load_words<D>(g.k, blk + share * (kv4_k_at(D, 1) - kv4_k_at(D, 0)) + at.k);
+        load_words<D>(g.v, blk + share * (kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0)) + at.v);
+        g.ks = *(const uint16_t *)(blk + share * 2 + at.ks);
+        const uint2 vs = *(const uint2 *)(blk + share * 8 + at.vs);
+        g.vs[0] = vs.x, g.vs[1] = vs.y;
     };
-    const auto stage = [&](PageShare<D> &g, int key0, int buf) {
-        if (takes_k) {
-            const h16x2 ks = as_h2((uint32_t)g.ks | (uint32_t)g.ks << 16);
+    const auto stage = [&](PageShare<D> &g, int it) {
+        const int key0 = (pb + HALVES * it + half) * KV4_PAGE;
+        u32x4 (*const to)[64] = lds.page[half][it & 1];
+        const h16x2 ks = as_h2((uint32_t)g.ks | (uint32_t)g.ks << 16);
 #pragma unroll
-            for (int j = 0; j < D / 32; j++) {
-                uint32_t k[4];
-                unpack8(un, g.k[j], ks, k);
-                lk[buf][share * (D / 32) + j][lane] = u32x4{k[0], k[1], k[2], k[3]};
-            }
+        for (int j = 0; j < D / 32; j++) {
+            uint32_t k[4];
+            unpack8(un, g.k[j], ks, k);
+            to[share * (D / 32) + j][lane] = u32x4{k[0], k[1], k[2], k[3]};
         }
-        if (takes_v) {
-            if (key0 + KV4_PAGE > g.held) mask_values(g.vs, key0 + 16 * kg + 4 * share, g.held);
+        if (key0 + KV4_PAGE > g.held) mask_values(g.vs, key0 + 16 * kg + 4 * share, g.held);
 #pragma unroll
-            for (int c = 0; c < D / 64; c++) {
-                uint32_t v0[4], v1[4];
-                unpack8(un, g.v[2 * c], as_h2(g.vs[0]), v0);
-                unpack8(un, g.v[2 * c + 1], as_h2(g.vs[1]), v1);
+        for (int c = 0; c < D / 64; c++) {
+            uint32_t v0[4], v1[4];
+            unpack8(un, g.v[2 * c], as_h2(g.vs[0]), v0);
+            unpack8(un, g.v[2 * c + 1], as_h2(g.vs[1]), v1);
 #pragma unroll
-                for (int n = 0; n < 4; n++)
-                    *((uint2 *)&lv[buf][share / 2 * (D / 16) + 4 * c + n][lane] + share % 2) = make_uint2(v0[n], v1[n]);
-            }
+            for (int n = 0; n < 4; n++)
+                *((uint2 *)&to[KF + share / 2 * (D / 16) + 4 * c + n][lane] + share % 2) = make_uint2(v0[n], v1[n]);
         }
     };
 
+    // a page too many for the second half is fetched as none and masked for every column
+    const int rounds = (pe - pb + HALVES - 1) / HALVES;
     PageShare<D> g;
-    if (pb < pe) {
-        fetch(g, pb);
-        stage(g, pb * KV4_PAGE, 0);
+    if (rounds > 0) {
+        fetch(g, 0);
+        stage(g, 0);
     }
     __syncthreads();
-    for (int page = pb; page < pe; page++) {
-        const int key0 = page * KV4_PAGE, buf = (page - pb) & 1;
-        if (page + 1 < pe) fetch(g, page + 1);
+    for (int it = 0; it < rounds; it++) {
+        const int key0 = (pb + HALVES * it + half) * KV4_PAGE;
+        const u32x4 (*const lk)[64] = lds.page[half][it & 1], (*const lv)[64] = lk + KF;
+        if (it + 1 < rounds) fetch(g, it + 1);
         // fragments are read from LDS in pairs, two pairs ahead of the products; the
         // reads stay where they are written (otherwise each is waited for by itself)
         f32x4 x[NC][4];
@@ -1143,11 +1151,11 @@ k_kv4_attn_rows(Kv4Attn a)
             to[0] = __builtin_bit_cast(half8, from[2 * n][lane]);
             to[1] = __builtin_bit_cast(half8, from[2 * n + 1][lane]);
         };
-        read(f[0], lk[buf], 0);
-        read(f[1], lk[buf], 1);
+        read(f[0], lk, 0);
+        read(f[1], lk, 1);
 #pragma unroll
         for (int n = 0; n < KF / 2; n++) {
-            if (n < KF / 2 - 2) read(f[(n + 2) % 3], lk[buf], n + 2);
+            if (n < KF / 2 - 2) read(f[(n + 2) % 3], lk, n + 2);
             __builtin_amdgcn_sched_barrier(DS_STAYS);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -1160,18 +1168,18 @@ k_kv4_attn_rows(Kv4Attn a)
                             f[n % 3][h], q[c].f[part][j], j == 0 && part == PARTS - 1 ? f32x4{0, 0, 0, 0} : x[c][k], 0, 0, 0);
             }
         }
-        read(f[0], lv[buf], 0);
-        read(f[1], lv[buf], 1);
+        read(f[0], lv, 0);
+        read(f[1], lv, 1);
         half8 p8[NC][PARTS][2];
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            if (key0 + KV4_PAGE - 1 > low[c] || (a.window && key0 <= high[c] - a.window))
-                mask_scores(x[c], key0, pos[c], a.window, kg);
+            if (key0 + KV4_PAGE - 1 > low[c] || (a.window && key0 <= high[c] - a.window) || key0 >= pe * KV4_PAGE)
+                mask_scores(x[c], key0, key0 < pe * KV4_PAGE ? pos[c] : -1, a.window, kg);
         }
         page_softmax<T, D, NC>(s, x, unit, p8);
 #pragma unroll
         for (int n = 0; n < VF / 2; n++) {
-            if (n < VF / 2 - 2) read(f[(n + 2) % 3], lv[buf], n + 2);
+            if (n < VF / 2 - 2) read(f[(n + 2) % 3], lv, n + 2);
             __builtin_amdgcn_sched_barrier(DS_STAYS);
 #pragma unroll
             for (int h = 0; h < 2; h++)
@@ -1179,33 +1187,55 @@ k_kv4_attn_rows(Kv4Attn a)
                 for (int c = 0; c < NC; c++)
                     add_values(s[c].o[(2 * n + h) % (D / 16)], f[n % 3][h], p8[c], (2 * n + h) / (D / 16));
         }
-        if (page + 1 < pe) stage(g, key0 + KV4_PAGE, buf ^ 1);
+        if (it + 1 < rounds) stage(g, it + 1);
         __syncthreads();
     }
+    float l[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        l[c] = add_xor32(add_xor16(s[c].l));
+        if (poisoned[c]) l[c] = __builtin_nanf("");
+        if (half) {                  // the pages are read: their place takes this half's result
+            const int cw = (share * NC + c) * 16 + r;
+            if (kg == 0) lds.half.m[cw] = s[c].m, lds.half.l[cw] = l[c];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 4)
+                    *(f32x4 *)&lds.half.o[cw][D / 4 * kg + D / 16 * e + i] =
+                        f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]};
+        }
+    }
+    if constexpr (HALVES == 2) __syncthreads();
+    if (half) return;
     const int64_t pi = ((int64_t)ti * a.cache.heads + hk) * a.splits + sp;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-        const int cw = (wave * NC + c) * 16 + r, col = t.cb + cw;
-        float l = add_xor32(add_xor16(s[c].l));
-        if (poisoned[c]) l = __builtin_nanf("");
+        const int cw = (share * NC + c) * 16 + r, col = t.cb + cw;
         if (col >= t.ncols) continue;
-        if (parts > 1) {
-            if (kg == 0) a.part[pi * 2 * W + cw] = s[c].m, a.part[(pi * 2 + 1) * W + cw] = l;
-            float *o = a.part + a.part_rows + (pi * W + cw) * D + D / 4 * kg;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int i = 0; i < D / 16; i += 4)
-                    *(f32x4 *)(o + D / 16 * e + i) = f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]};
-        } else {
-            T *o = (T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + D / 4 * kg;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // a column that saw nothing has o = 0
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int i = 0; i < D / 16; i += 4)
-                    store4(o + D / 16 * e + i, f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]} * inv, a.vec);
+        float M = s[c].m, f1 = 1.0f, f2 = 0.0f, sum = l[c];
+        if constexpr (HALVES == 2) {
+            const float m2 = lds.half.m[cw];
+            M = fmaxf(s[c].m, m2);
+            f1 = s[c].m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[c].m - M);
+            f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - M);
+            sum = l[c] * f1 + lds.half.l[cw] * f2;
         }
+        const float by = parts > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;   // a column that saw nothing has o = 0
+        if (parts > 1 && kg == 0) a.part[pi * 2 * W + cw] = M, a.part[(pi * 2 + 1) * W + cw] = sum;
+        float *part = a.part + a.part_rows + (pi * W + cw) * D + D / 4 * kg;
+        T *out = (T *)a.out + (t.r0 + col / a.group) * a.out_stride + (hk * a.group + col % a.group) * D + D / 4 * kg;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int i = 0; i < D / 16; i += 4) {
+                f32x4 o = f32x4{s[c].o[i][e], s[c].o[i + 1][e], s[c].o[i + 2][e], s[c].o[i + 3][e]} * (f1 * by);
+                if constexpr (HALVES == 2) o += *(const f32x4 *)&lds.half.o[cw][D / 4 * kg + D / 16 * e + i] * (f2 * by);
+                if (parts > 1)
+                    *(f32x4 *)(part + D / 16 * e + i) = o;
+                else
+                    store4(out + D / 16 * e + i, o, a.vec);
+            }
     }
 }
 
@@ -1256,34 +1286,34 @@ static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return k
 // How a call is cut: columns of a tile, pages of a workgroup, the most
 // workgroups of a tile.
 //
-// The wide tiles unpack a page once for 128 columns, but a workgroup's way
-// through its pages takes longer (1.9 us a page, 16 columns 0.9), so they pay
-// where there are many: 32 sequences of 2048 positions, bf16, take with 16
-// columns / wide 51 / 63 us for 32 rows each, 94 / 67 for 64, 179 / 96 for 128,
-// but 8 sequences 51 / 78 for 128 rows; of 400 positions, 64 sequences 22 / 27
-// for 16 rows, 36 / 31 for 32, 64 / 39 for 64.
+// The wide tiles unpack a page once for 128 columns, but cost the same for a
+// few and take a page longer (1.9 us, 16 columns 0.9): they pay where three
+// tiles of 16 columns do not hold a sequence's and there are enough to fill the
+// card.  16 columns / wide, in us, bf16, 8 kv heads of two: 64 sequences of 400
+// positions with 16, 24, 28, 64 rows each 23 / 29, 29 / 29, 36 / 30, 63 / 39; of
+// 2048 positions, 8 sequences of 64, 128, 256 rows 28 / 52, 48 / 50, 90 / 54, 32
+// sequences of 28, 32, 40, 128 rows 50 / 51, 52 / 52, 62 / 53, 174 / 93; one of
+// 4000 positions with 2000 rows 136 / 86.  f32 rows change over at the same sizes.
 //
 // Splitting a tile's pages costs a second kernel (5 us, and its launch), and
 // pays where workgroups are few: 16 sequences of 16000 positions in 1024 parts 45
 // us, in 256 81; 64 of 1365 to 4096, 512 workgroups, 53 whole and 61 in two.  So
 // up to 16 pages, four for each of a workgroup's waves, stay whole (one sequence
-// of 700 11 us, in two 15), and so do shorter ones than 64 pages (wide: 128) where
-// the card is full without; longer ones are split for the sake of the shorter
-// ones beside them.
+// of 700 11 us, in two 15), and so do shorter ones than 64 pages where the card
+// is full without, and all up to 128 on wide tiles (16 sequences of 64 rows on
+// 2048 positions 51 us, in two 72); longer ones are split for the sake of the
+// shorter ones beside them.
 Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
 {
     Kv4Cut c{};
     const int64_t cols = n_seqs ? rows * group / n_seqs : 0;     // of an average sequence
-    const bool wide = cols >= 48 && rows * group * kv_heads >= 24576;
+    const bool wide = cols > 48 && rows * group * kv_heads > 16384;
     c.width = wide ? KV4_WIDE : KV4_W;
     const int64_t items = std::max<int64_t>(attn_tiles(rows, n_seqs, group, c.width) * kv_heads, 1);
     int64_t pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
     if (window) pages = std::min<int64_t>(pages, ((int64_t)window + c.width - 2) / KV4_PAGE + 2);
-    int64_t per;
-    if (wide)
-        per = items >= 256 ? 128 : std::max<int64_t>(items * pages / 512, 8);
-    else
-        per = items >= 512 ? 64 : pages <= 16 ? 16 : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);
+    int64_t per = 128;
+    if (!wide) per = items >= 512 ? 64 : pages <= 16 ? 16 : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);
     per = std::max<int64_t>(per, (pages + 63) / 64);
     c.chunk = (int)std::min<int64_t>(per, INT32_MAX / KV4_PAGE);
     c.splits = (int)std::max<int64_t>(1, (pages + per - 1) / per);
@@ -1300,19 +1330,23 @@ static hipError_t launch_attn(const Kv4Attn &a, int width, hipStream_t s)
 {
     const unsigned tiles = (unsigned)attn_tiles(a.rows, a.n_seqs, a.group, width);
     const bool wide = width == KV4_WIDE;
-    constexpr int NC = 2;
-    if (wide)
-        hipLaunchKernelGGL((k_kv4_attn_rows<T, D, NC>), dim3(tiles * a.cache.heads, a.splits), dim3(KV4_WIDE / NC * 4), 0, s, a);
+    const dim3 grid(tiles * a.cache.heads, a.splits);
+    // about how many tiles there are: sequences of the average length
+    const int64_t cols = ((int64_t)a.rows * a.group + a.n_seqs - 1) / a.n_seqs;
+    if (wide && (cols + width - 1) / width * a.n_seqs * a.cache.heads * a.splits <= 256)
+        hipLaunchKernelGGL((k_kv4_attn_rows<T, D, 2>), grid, dim3(512), 0, s, a);
+    else if (wide)
+        hipLaunchKernelGGL((k_kv4_attn_rows<T, D, 1>), grid, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv4_attn<T, D>), dim3(tiles * a.cache.heads, a.splits), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv4_attn<T, D>), grid, dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     // a workgroup a column of an average sequence's tile
-    const unsigned cols = (unsigned)std::min<int64_t>(width, ((int64_t)a.rows * a.group + a.n_seqs - 1) / a.n_seqs);
+    const dim3 join(tiles * a.cache.heads, (unsigned)std::min<int64_t>(width, cols));
     if (wide)
-        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_WIDE>), dim3(tiles * a.cache.heads, cols), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_WIDE>), join, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_W>), dim3(tiles * a.cache.heads, cols), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv4_attn_join<T, D, KV4_W>), join, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -54,28 +54,28 @@ def _elsewhere(name, t, device):
 
 def _vector(name, t, n, dtype, device):
     """The address of a contiguous vector of n values of that type."""
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: contiguous {dtype} [{n}] expected, got {t.dtype} {list(t.shape)}")
     if t.get_device() != device:
         raise _elsewhere(name, t, device)
     return t.data_ptr()
 
 
-def _rows(name, t, rows, heads, dim, dtype, device):
-    """[rows][heads][dim] with whole heads next to each other: the row stride."""
-    shape = t.shape
-    if t.dim() != 3 or shape[0] != rows or shape[1] != heads or shape[2] != dim:
-        raise ValueError(f"{name}: [{rows}][{heads}][{dim}] expected, got {list(shape)}")
+def _rows(name, t, shape, dtype, device):
+    """shape = (rows, heads, dim) with whole heads next to each other: the row stride."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: {list(shape)} expected, got {list(t.shape)}")
     if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, not {dtype}")
     if t.get_device() != device:
         raise _elsewhere(name, t, device)
+    rows, heads, dim = shape
     if rows == 0:
         return heads * dim
-    s = t.stride()
-    if s[2] != 1 or (heads > 1 and s[1] != dim):
+    row, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != dim):
         raise ValueError(f"{name}: the heads of a row must lie next to each other")
-    return s[0] if rows > 1 else heads * dim
+    return row if rows > 1 else heads * dim
 
 
 def _table(t, n, device):
@@ -94,15 +94,14 @@ class Kv4Cache:
     def __init__(self, pages, n_kv_heads, head_dim):
         if _torch is None:
             _load()
-        size, inner = n_kv_heads * 72 * head_dim, 1
-        shape, strides = pages.shape, pages.stride()
-        n = shape[0] if shape else 0
+        size, shape, strides = n_kv_heads * 72 * head_dim, pages.shape, pages.stride()
+        n, inner = shape[0] if shape else 0, 1
         for d in range(len(shape) - 1, 0, -1):
-            if shape[d] > 1 and strides[d] != inner:
+            if strides[d] != inner and shape[d] > 1:
                 inner = -1
                 break
             inner *= shape[d]
-        if pages.dtype is not _torch.uint8 or len(shape) < 2 or inner != size:
+        if inner != size or pages.dtype is not _torch.uint8 or len(shape) < 2:
             raise ValueError(f"pages: uint8 [n][{size}] expected, got {pages.dtype} {list(shape)}")
         self.pages, self.n_kv_heads, self.head_dim = pages, n_kv_heads, head_dim
         self.device = pages.get_device()
@@ -169,40 +168,42 @@ def qk_norm_rope(self, q, k, positions=None, cos=None, sin=None, q_norm=None, k_
     if _torch is None:
         _load()
     device, dtype = self.device, q.dtype
-    rows, heads, dim = q.shape
-    kv_heads = k.shape[1]
+    rows, heads, dim = shape = q.shape
+    kv_heads = k.shape[1] if k.dim() == 3 else 0
+    k_shape = (rows, kv_heads, dim)
     code = _code("q", q)
-    q_stride = _rows("q", q, rows, heads, dim, dtype, device)
-    k_stride = _rows("k", k, rows, kv_heads, dim, dtype, device)
+    q_stride, k_stride = _rows("q", q, shape, dtype, device), _rows("k", k, k_shape, dtype, device)
     if q_out is None:
         q_out, qo_stride = _torch.empty_like(q, memory_format=_torch.contiguous_format), heads * dim
     else:
-        qo_stride = _rows("q_out", q_out, rows, heads, dim, dtype, device)
+        qo_stride = _rows("q_out", q_out, shape, dtype, device)
     if k_out is None and cache is None:
         k_out = _torch.empty_like(k, memory_format=_torch.contiguous_format)
-    ko, ko_stride = (0, 0) if k_out is None else (k_out.data_ptr(), _rows("k_out", k_out, rows, kv_heads, dim, dtype, device))
+    ko, ko_stride = (0, 0) if k_out is None else (k_out.data_ptr(), _rows("k_out", k_out, k_shape, dtype, device))
     at = cos_at = sin_at = most = vp = v_stride = desc = slots_at = 0
     if positions is not None:
         if cos is None or sin is None:
             raise ValueError("positions need cos and sin")
-        most = cos.shape[0]
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype is not _torch.float32 or t.dim() != 2 or t.shape[0] != most or t.shape[1] != dim // 2 or not t.is_contiguous():
-                raise ValueError(f"{name}: contiguous float32 [{most}][{dim // 2}] expected, got {t.dtype} {list(t.shape)}")
-            if t.get_device() != device:
-                raise _elsewhere(name, t, device)
+        most, f32 = cos.shape[0], _torch.float32
+        table = (most, dim // 2)
+        if cos.shape != table or sin.shape != table or cos.dtype is not f32 or sin.dtype is not f32 or \
+                not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError(f"cos and sin: contiguous float32 [max_pos][{dim // 2}] expected")
+        if cos.get_device() != device or sin.get_device() != device:
+            raise _elsewhere("cos or sin", cos if cos.get_device() != device else sin, device)
         at, cos_at, sin_at = _vector("positions", positions, rows, _torch.int32, device), cos.data_ptr(), sin.data_ptr()
     if cache is not None:
         if v is None or slots is None:
             raise ValueError("a cache needs v and slots")
         if cache.device != device:
             raise _elsewhere("the cache", cache.pages, device)
-        vp, v_stride, desc = v.data_ptr(), _rows("v", v, rows, kv_heads, dim, dtype, device), cache.address
+        vp, v_stride, desc = v.data_ptr(), _rows("v", v, k_shape, dtype, device), cache.address
         slots_at = _vector("slots", slots, rows, _torch.int64, device)
+    f16 = _torch.float16
     a = _POST.pack(code, heads, kv_heads, dim, rows, q.data_ptr(), k.data_ptr(), vp, q_stride, k_stride, v_stride,
                    q_out.data_ptr(), ko, qo_stride, ko_stride,
-                   0 if q_norm is None else _vector("q_norm", q_norm, dim, _torch.float16, device),
-                   0 if k_norm is None else _vector("k_norm", k_norm, dim, _torch.float16, device),
+                   0 if q_norm is None else _vector("q_norm", q_norm, dim, f16, device),
+                   0 if k_norm is None else _vector("k_norm", k_norm, dim, f16, device),
                    eps, 0, cos_at, sin_at, most, at, desc, slots_at)
     rc = self.lib.qtts_qk_norm_rope(self.h, a, _stream(device), 0)
     if rc:
@@ -243,11 +244,12 @@ def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, m
     if q.dim() != 3:
         raise ValueError(f"q: [rows][heads][{dim}] expected, got {list(q.shape)}")
     rows, heads = q.shape[0], q.shape[1]
-    code, q_stride = _code("q", q), _rows("q", q, rows, heads, dim, dtype, device)
+    shape = (rows, heads, dim)
+    code, q_stride = _code("q", q), _rows("q", q, shape, dtype, device)
     if out is None:
         out, out_stride = _torch.empty_like(q, memory_format=_torch.contiguous_format), heads * dim
     else:
-        out_stride = _rows("out", out, rows, heads, dim, dtype, device)
+        out_stride = _rows("out", out, shape, dtype, device)
     columns = table.shape[1] if table.dim() == 2 else 0
     head = (code, heads, rows, q.data_ptr(), out.data_ptr(), q_stride, out_stride, cache.address, n, columns,
             _vector("row_start", row_start, n + 1, i32, device), _vector("lengths", lengths, n, i32, device), table.data_ptr(),

@@ -105,14 +105,14 @@ def attention(q, pool, table, row_start, lengths, scale, window):
             if pos < 0:
                 out[r] = 0
                 continue
-            for h in range(heads):
-                kk, vv = k[lo:pos + 1, h // G], v[lo:pos + 1, h // G]
-                s = kk @ q[r, h] * scale
-                w = np.exp(s - s.max())
-                w /= w.sum()
+            for kv in range(heads // G):
+                h, kk, vv = slice(kv * G, kv * G + G), k[lo:pos + 1, kv], v[lo:pos + 1, kv]
+                s = q[r, h] @ kk.T * scale
+                w = np.exp(s - s.max(1, keepdims=True))
+                w /= w.sum(1, keepdims=True)
                 out[r, h] = w @ vv
-                mag[r, h, :, 0], mag[r, h, :, 1] = w @ np.abs(vv), w.max() * np.abs(vv).sum(0)
-                big[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale)
+                mag[r, h, :, 0], mag[r, h, :, 1] = w @ np.abs(vv), w.max(1)[:, None] * np.abs(vv).sum(0)
+                big[r, h] = (np.abs(q[r, h]) @ np.abs(kk).T).max(1) * abs(scale)
     return out, mag, big
 
 

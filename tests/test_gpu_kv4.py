@@ -506,6 +506,89 @@ def test_attention_no_rows_and_no_sequences(ctx):
     assert bool((out == 2).all())
 
 
+# More than 48 columns a sequence and 16384 in all take tiles of 128 columns.
+
+# sequences, rows of each, query heads, kv heads, head width
+WIDE = [([150, 257, 131], [150, 131, 128], 41, 1, 128),           # 137 tiles: two groups of waves a tile
+        ([300, 0, 64, 200], [190, 0, 1, 180], 60, 2, 64),
+        ([400, 450], [400, 400], 66, 2, 128),                    # 414 tiles: one
+        ([65, 500, 129], [65, 480, 1], 98, 1, 64)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("window", [0, 72])
+@pytest.mark.parametrize("lengths,fresh,H,HK,D", WIDE)
+def test_attention_wide_tiles(ctx, kind, window, lengths, fresh, H, HK, D):
+    say("wide", kind, window, lengths, H, HK, D)
+    out = torch.full((sum(fresh) + 3, H, D), 5.0, dtype=TYPES[kind], device=DEV)
+    attend(ctx, Served(lengths, HK, D, seed=H), fresh, H, kind, window=window, extra=3, out=out, pad=3 if window else 0)
+    assert bool((out[sum(fresh):] == 5).all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attention_wide_tiles_split(ctx, kind):
+    """Pages past a workgroup's 128 go to others; the short sequence beside is
+    not split."""
+    say("wide split", kind)
+    attend(ctx, Served([8700, 50], 1, 64, seed=30), [70, 50], 140, kind)
+
+
+@pytest.mark.parametrize("rows", [140, 420])
+def test_attention_wide_tiles_sharp_and_flat(ctx, rows):
+    for scale in (-0.5, 1e-4, 3.0):
+        say("wide", rows, scale)
+        attend(ctx, Served([420], 1, 64, seed=31), [rows], 120, "f32", scale=scale)
+
+
+@pytest.mark.parametrize("rows", [140, 420])
+@pytest.mark.parametrize("entry", [-1, 2 ** 31 - 1])
+def test_attention_wide_tiles_bad_pages(ctx, rows, entry):
+    """NaN for the rows that see the page, and for no other."""
+    say("wide bad page", rows, entry)
+    sv = Served([420], 1, 64, seed=32)
+    table = sv.table.copy()
+    table[0, 5] = entry                  # positions 320 .. 383
+    q = torch.randn((rows, 120, 64), generator=torch.Generator().manual_seed(3)).to(DEV)
+    pos = np.arange(420 - rows, 420)
+    for window in (0, 10):
+        got = host(ctx.kv4_attention(q, sv.cache, i32(table), i32([0, rows]), i32([420]), window=window))
+        want, mag, big = kv4_ref.attention(host(q), sv.pool, sv.table, [0, rows], [420], np.float64(np.float32(1 / 8)), window)
+        sees = (pos >= 320) & ((window == 0) | (pos - window < 383))
+        assert np.isnan(got[sees]).all() and sees.any() and not sees.all()
+        compare(got[~sees], want[~sees], mag[~sees], big[~sees], "f32", [420])
+
+
+@pytest.mark.parametrize("rows,HK", [(150, 1), (450, 1)])
+def test_attention_wide_tiles_nan_and_empty_rows(ctx, rows, HK):
+    """Rows before the sequence are zero; a NaN in a position reaches the rows
+    that see it."""
+    sv = Served([130], HK, 64, seed=33)
+    slot = lambda p: sv.table[0][p // PAGE] * PAGE + p % PAGE
+    k, v = sv.pool.get([slot(70)])
+    v[:] = np.nan
+    sv.pool.put([slot(70)], k, v)
+    sv.cache.pages.copy_(torch.as_tensor(sv.pool.b))
+    q = torch.randn((rows, 120, 64), generator=torch.Generator().manual_seed(2)).to(DEV)
+    for window in (0, 20):
+        got = host(ctx.kv4_attention(q, sv.cache, i32(sv.table), i32([0, rows]), i32([130]), window=window))
+        want, mag, big = kv4_ref.attention(host(q), sv.pool, sv.table, [0, rows], [130], np.float64(np.float32(1 / 8)), window)
+        bad = np.isnan(want).any(-1)
+        assert bad.any() and not bad.all() and np.array_equal(np.isnan(got).all(-1), bad)
+        assert (got[:rows - 130] == 0).all()
+        compare(got[~bad], want[~bad], mag[~bad], big[~bad], "f32", [130])
+
+
+def test_attention_wide_tiles_short_table_and_bad_sums(ctx):
+    sv = Served([128], 1, 64, seed=34, columns=2)
+    q = torch.randn((150, 120, 64), generator=torch.Generator().manual_seed(4)).to(DEV)
+    got = ctx.kv4_attention(q, sv.cache, i32(sv.table), i32([0, 150]), i32([130]))
+    assert not torch.isnan(got[:148]).any() and torch.isnan(got[148:]).all()
+    for row_start, length in (([0, 151], 64), ([150, 0], 64), ([-5, 150], 64), ([0, 150], -1), ([0, 150], 2 ** 31 - 1)):
+        out = torch.full_like(q, 9.0)
+        ctx.kv4_attention(q, sv.cache, i32(sv.table), i32(row_start), i32([length]), out=out)
+        assert bool((out == 9).all())
+
+
 def test_many_sequences_find_their_tiles(ctx):
     """4097 sequences, some without rows: every row must find its own."""
     r = np.random.default_rng(15)
