@@ -574,11 +574,48 @@ struct AttnTile {
     int b, r0, n, len, cb, ncols;
 };
 
+// Sums over lanes 0 .. l of the wave, in each lane l.
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8: sums over rows of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15: the row before, to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast 31: the first half, to the second
+    return v;
+}
+
+// Workgroups a round: about as many as the card has CUs.
+constexpr int ROUND = 256;
+
+// Tiles in descending order of their pages, `all` of them of which the card
+// takes `round` at once: the place that number i has among them.  Where there
+// are no more than two rounds, a CU gets a second tile while it still has its
+// first, the smaller ones beside the larger: the first round begins with those
+// that are to share a CU, and the second goes upwards.
+__device__ __forceinline__ int tile_place(int i, int all, int round)
+{
+    if (all <= round || all > 2 * round) return i;
+    const int shared = all - round;
+    return i >= round ? all - 1 - (i - round) : i < shared ? round - shared + i : i - shared;
+}
+
 // The tile with number ti, found by the whole wave: first its block of 64
 // sequences (each round, 64 lanes look at 64 evenly spaced ones), then the
 // sequence by a sum over the block's.  One load of latency for 64 sequences,
 // two for 4096.  False where no tile has this number, and for row sums that
 // are none.
+//
+// Where there are more workgroups than CUs, a block's tiles are numbered by
+// the pages that they see, the most first: a lane counts its sequence's tiles
+// of p pages or more (a sequence's later tiles see more), and p is found by
+// bisection, in 1 us.  64 sequences of 1365 to 4096 positions in no order take
+// 37 us, numbered in the order of the sequences 46 (of 667 to 2000 24 / 27, 256 of
+// 1365 to 4096 158 / 162); four prompts of 500 to 1000 rows on 667 to 2000 60 / 69.
+// Not for tiles of fewer pages (256 sequences of up to 500 positions 35 / 33) and
+// not where they are cut into parts of less than 64 pages, which are even already
+// (48 sequences of up to 4096 40 / 38).
 __device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnTile &t)
 {
     const int lane = threadIdx.x & 63;
@@ -596,16 +633,34 @@ __device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnT
     // what a lane's sequence is comes with the same wait as its rows
     const int b = min(lo + lane, a.n_seqs), r0 = a.row_start[b], r1 = a.row_start[min(b + 1, a.n_seqs)];
     const int len = a.lengths[min(b, a.n_seqs - 1)];
-    const int s0 = min(max(r0, 0), a.rows), s1 = min(max(r1, 0), a.rows);
-    const int tiles = max(((s1 - s0) * a.group + W - 1) / W, 0);
-    int end = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int below = __shfl_up(end, d);
-        if (lane >= d) end += below;
+    const int s0 = min(max(r0, 0), a.rows), s1 = min(max(r1, 0), a.rows), n = max(s1 - s0, 0);
+    const int tiles = (n * a.group + W - 1) / W;
+    int rel = ti - (int)kv4_first_tile(__builtin_amdgcn_readlane(s0, 0), a.group, lo, W);
+    int end = wave_scan(tiles), first = end - tiles, skip = 0;
+    const int all = __builtin_amdgcn_readlane(end, 63);
+    if (rel < 0 || rel >= all) return false;
+    const int seen = min(max(len, 0), INT32_MAX - KV4_PAGE);
+    // more pages than any tile sees: a length rounded to f32 is off by a page at most
+    const int bound = min((int)wave_max_dpp(n ? (float)seen : 0.0f) / KV4_PAGE + 4, a.max_pages + 1);
+    if (all * a.cache.heads > ROUND && a.chunk >= 64 && bound > (W == KV4_W ? 20 : 8)) {
+        rel = tile_place(rel, all, max(ROUND / a.cache.heads, 1));
+        // tiles of p + 1 pages or more: those of the rows that see position 64 p
+        const auto count = [&](int p) {
+            const int at = p * KV4_PAGE, row = max(at - (seen - n), 0);
+            return at >= seen ? 0 : tiles - (int)((uint32_t)(row * a.group) / (uint32_t)W);
+        };
+        int p = 0, more = bound;
+        while (more - p > 1) {
+            const int mid = (p + more) / 2;
+            if (__builtin_amdgcn_readlane(wave_scan(count(mid - 1)), 63) > rel) p = mid; else more = mid;
+        }
+        // those of p pages: of each sequence the tiles before the `skip` last
+        skip = more > a.max_pages ? 0 : count(more - 1);
+        rel -= __builtin_amdgcn_readlane(wave_scan(skip), 63);
+        const int here = (p ? count(p - 1) : tiles) - skip;
+        end = wave_scan(here), first = end - here;
     }
-    const int64_t rel = ti - kv4_first_tile(__builtin_amdgcn_readlane(s0, 0), a.group, lo, W);
-    const uint64_t m = __ballot(rel >= end - tiles && rel < end);
+    const uint64_t m = __ballot(rel >= first && rel < end);
     if (!m) return false;
     const int at = __ffsll((unsigned long long)m) - 1;
     t.b = lo + at;
@@ -615,7 +670,9 @@ __device__ __forceinline__ bool find_tile(const Kv4Attn &a, int ti, int W, AttnT
     if (t.r0 < 0 || last > a.rows || last <= t.r0 || t.len < 0 || t.len > INT32_MAX - KV4_PAGE) return false;
     t.n = last - t.r0;
     t.ncols = t.n * a.group;
-    t.cb = (int)(rel - __builtin_amdgcn_readlane(end - tiles, at)) * W;
+    // from the last of a sequence's tiles to its first
+    const int j = __builtin_amdgcn_readlane(tiles - 1 - skip, at) - (rel - __builtin_amdgcn_readlane(first, at));
+    t.cb = j * W;
     return t.cb < t.ncols;
 }
 
@@ -1048,8 +1105,8 @@ constexpr int DS_STAYS = 0x47F;      // sched_barrier: all but LDS instructions 
 // other page, joined at the end.  The longest tile's way is half as long, and
 // each SIMD has two waves to take turns.  2048 positions, sequences of 64 rows, in
 // us with four waves / eight: 16 sequences (128 tiles) 65 / 51, 32 70 / 59, 64 104 /
-// 114, and four prompts of 500 to 1000 rows (376 tiles) 79 / 84: there two
-// workgroups of four share a CU more evenly.
+// 114, and four prompts of 500 to 1000 rows (376 tiles) 79 / 84 (61 with the
+// tiles in order): there two workgroups of four share a CU.
 template <class T, int D, int HALVES>
 __global__ void __launch_bounds__(256 * HALVES, 2)
 k_kv4_attn_rows(Kv4Attn a)
@@ -1064,8 +1121,7 @@ k_kv4_attn_rows(Kv4Attn a)
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kg = lane >> 4, share = wave & 3, half = HALVES == 2 ? wave >> 2 : 0;
-    // the last tiles of a sequence see the most: they go first
-    const int bx = gridDim.x - 1 - blockIdx.x, ti = bx / a.cache.heads, hk = bx % a.cache.heads, sp = blockIdx.y;
+    const int ti = blockIdx.x / a.cache.heads, hk = blockIdx.x % a.cache.heads, sp = blockIdx.y;
     AttnTile t;
     if (!find_tile(a, ti, W, t)) return;
     int minpos, maxpos, pg0, pages;
@@ -1297,7 +1353,7 @@ static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return k
 //
 // Splitting a tile's pages costs a second kernel (5 us, and its launch), and
 // pays where workgroups are few: 16 sequences of 16000 positions in 1024 parts 45
-// us, in 256 81; 64 of 1365 to 4096, 512 workgroups, 53 whole and 61 in two.  So
+// us, in 256 81; 64 of 1365 to 4096, 512 workgroups, 45 whole and 61 in two.  So
 // up to 16 pages, four for each of a workgroup's waves, stay whole (one sequence
 // of 700 11 us, in two 15), and so do shorter ones than 64 pages where the card
 // is full without, and all up to 128 on wide tiles (16 sequences of 64 rows on
@@ -1323,8 +1379,8 @@ Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t m
 
 // The kv heads of a tile are neighbours in the grid: workgroups go round the
 // XCDs one by one, and so each XCD gets as much of a long sequence as of a
-// short one (64 sequences of 1365 to 4096 positions: 53 us, with the tiles as
-// neighbours 59).
+// short one (64 sequences of 1365 to 4096 positions in the order given: 53 us, with
+// the tiles as neighbours 59).
 template <class T, int D>
 static hipError_t launch_attn(const Kv4Attn &a, int width, hipStream_t s)
 {

@@ -606,6 +606,45 @@ def test_many_sequences_find_their_tiles(ctx):
     assert (np.abs(got - want) <= want * 2.0 ** -21).all()
 
 
+# More than 256 workgroups: tiles are taken in order of their pages, if there
+# are more than 16 of them (wide tiles: 4).  Sequences, kv heads, query heads,
+# most rows, window, longest.
+ORDERED = [("bf16", 64, 8, 16, 1, 0, 1100), ("f32", 60, 9, 18, 1, 0, 1100), ("f16", 40, 16, 16, 3, 100, 1100), ("f32", 130, 4, 68, 2, 0, 1100),
+           ("bf16", 300, 2, 4, 1, 0, 1100), ("f32", 20, 16, 320, 9, 70, 1100), ("bf16", 9, 4, 480, 60, 0, 500), ("f32", 33, 8, 8, 3, 0, 260)]
+
+
+@pytest.mark.parametrize("kind,seqs,HK,H,most,window,longest", ORDERED)
+def test_attention_ordered_tiles(ctx, kind, seqs, HK, H, most, window, longest):
+    """Lengths in no order, some equal, some empty: every row is written, once."""
+    say("ordered", kind, seqs, HK, H, most, window)
+    r = np.random.default_rng(seqs)
+    lengths = (r.integers(0, longest, seqs) // r.choice([1, 8, 64], seqs)).tolist()
+    lengths[seqs // 2] = longest
+    fresh = r.integers(0 if most > 1 else 1, most + 1, seqs).tolist()
+    rows = sum(fresh)
+    out = torch.full((rows + 2, H, 64), 5.0, dtype=TYPES[kind], device=DEV)
+    attend(ctx, Served(lengths, HK, 64, seed=seqs), fresh, H, kind, window=window, extra=2, out=out)
+    assert bool((out[rows:] == 5).all())
+
+
+def test_attention_ordered_tiles_with_bad_sequences(ctx):
+    """Lengths that are none, in the midst of others: their rows stay, the
+    others' are written."""
+    lengths = np.random.default_rng(1).integers(1, 1100, 64) // 2
+    lengths[7] = 1100
+    sv = Served(lengths.tolist(), 8, 64, seed=41)
+    given = lengths.copy()
+    given[[3, 20]], given[41], given[50] = -7, 2 ** 31 - 1, 2 ** 31 - 70
+    q = torch.randn((64, 8, 64), generator=torch.Generator().manual_seed(6)).to(DEV)
+    out = torch.full_like(q, 9.0)
+    ctx.kv4_attention(q, sv.cache, i32(sv.table), i32(np.arange(65)), i32(given), out=out, max_len=1100)
+    got, bad = host(out), np.isin(np.arange(64), [3, 20, 41])
+    assert (got[bad] == 9).all() and np.isnan(got[50]).all()
+    bad[50] = True
+    want, mag, big = kv4_ref.attention(host(q), sv.pool, sv.table, np.arange(65), lengths, 0.125, 0)
+    compare(got[~bad], want[~bad], mag[~bad], big[~bad], "f32", lengths)
+
+
 def test_pages_far_into_a_large_pool(ctx):
     """Offsets beyond 32 bits, and layers interleaved page by page."""
     HK, D = 8, 128
