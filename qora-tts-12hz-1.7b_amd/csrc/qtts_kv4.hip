@@ -257,11 +257,11 @@ __device__ __forceinline__ void norm_rope(Head<F> &x, bool norm, f32x4 ga, f32x4
 // step is -1/8 of the value of largest magnitude, rounded to f16 and then to
 // 8 significant bits; the nearest step's number, halves to even, plus 8.
 //
-// In f32 where that decides as f64 does, else in f64: rounding to f32 keeps the
-// order of values, so only two extremes that it makes equal have to be looked at
-// again, and the quotient (at most 16, off by 2^-22 of it from x, the reciprocal
-// and the product) only next to a half.  In f64 throughout, the quantisation of
-// 4001 rows of 16 heads took 22.3 us instead of 18.7.
+// In f32 where that decides as f64 does: rounding to f32 keeps the order of
+// values, so only two extremes that it makes equal have to be looked at again,
+// and the quotient (at most 16, off by 2^-22 of it from x, the reciprocal and the
+// product) only next to a half.  In f64 throughout, the kernel took 22.3 us for 4001
+// rows of 16 heads instead of 17.2.
 template <class F>
 __device__ __forceinline__ uint32_t quantise(const F (&x)[4], uint16_t &scale)
 {
@@ -297,8 +297,14 @@ __device__ __forceinline__ uint32_t quantise(const F (&x)[4], uint16_t &scale)
     if (far > 0.49999f) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const double q = fmin(fmax((double)x[i], -65280.0), 65280.0) / (double)d;
-            code[i] = (float)fmin(fmax(rint(q) + 8.0, 0.0), 15.0);
+            // on which side of the half next to it x / d lies: h d has 13 bits, so the
+            // difference has the right sign and is zero only at a tie
+            const float q = v[i] * inv, r = __builtin_rintf(q), h = q < r ? r - 0.5f : r + 0.5f;
+            const F e = fma((F)-h, (F)d, x[i]);
+            const uint32_t up = __builtin_bit_cast(uint32_t, (float)e) ^ __builtin_bit_cast(uint32_t, d);    // its sign: e / d's
+            const float near = h + __builtin_copysignf(0.5f, __builtin_bit_cast(float, up)), even = __builtin_rintf(h);
+            const float n = e == 0 ? even : near;
+            code[i] = __builtin_amdgcn_fmed3f(n + 8.0f, 0.0f, 15.0f);
         }
     }
     return (uint32_t)fmaf(4096.0f, code[3], fmaf(256.0f, code[2], fmaf(16.0f, code[1], code[0])));
@@ -306,9 +312,10 @@ __device__ __forceinline__ uint32_t quantise(const F (&x)[4], uint16_t &scale)
 
 // D / 8 lanes take one row's query heads of one kv head, that kv head's key
 // and, with a cache, its value: the angles are loaded once for all of them.
-// ONE_ROW: a wave's heads are of one row (the kv heads are a multiple of those
-// that a wave holds), whose addresses are then scalar.
-template <class T, int D, bool STORE, bool ONE_ROW>
+// FAST: a wave's heads are of one row (the kv heads are a multiple of those
+// that a wave holds), whose addresses are then scalar, and four elements move at
+// once everywhere.
+template <class T, int D, bool STORE, bool FAST>
 __global__ void __launch_bounds__(256)
 k_qk_norm_rope(QkNormRope a)
 {
@@ -316,7 +323,7 @@ k_qk_norm_rope(QkNormRope a)
     const int lane = threadIdx.x & 63, j = lane % L;
     const int first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * HEADS;
     int row, hk;
-    if constexpr (ONE_ROW) {
+    if constexpr (FAST) {
         row = __builtin_amdgcn_readfirstlane(first / a.kv_heads);
         hk = first - row * a.kv_heads + lane / L;
     } else {
@@ -324,7 +331,7 @@ k_qk_norm_rope(QkNormRope a)
         hk = (first + lane / L) % a.kv_heads;
     }
     if (row >= a.rows) return;
-    const bool vec = a.vec;
+    const bool vec = FAST || a.vec;
     const uint32_t at = hk * D + 4 * j, up = at + D / 2;     // a lane's columns of k and v
     const int32_t pos = a.positions ? a.positions[row] : 0;
 
@@ -408,21 +415,21 @@ k_qk_norm_rope(QkNormRope a)
     }
 }
 
-template <class T, int D, bool ONE_ROW>
+template <class T, int D, bool FAST>
 static void launch_qk_as(const QkNormRope &a, bool store, hipStream_t s)
 {
     const int64_t heads = (int64_t)a.rows * a.kv_heads, per = 256 / (D / 8);
     const dim3 grid((unsigned)((heads + per - 1) / per));
     if (store)
-        hipLaunchKernelGGL((k_qk_norm_rope<T, D, true, ONE_ROW>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, true, FAST>), grid, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_qk_norm_rope<T, D, false, ONE_ROW>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_qk_norm_rope<T, D, false, FAST>), grid, dim3(256), 0, s, a);
 }
 
 template <class T, int D>
 static hipError_t launch_qk(const QkNormRope &a, bool store, hipStream_t s)
 {
-    if (a.kv_heads % (512 / D) == 0)
+    if (a.vec && a.kv_heads % (512 / D) == 0)
         launch_qk_as<T, D, true>(a, store, s);
     else
         launch_qk_as<T, D, false>(a, store, s);
@@ -1366,7 +1373,7 @@ Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t m
     const bool wide = cols > 48 && rows * group * kv_heads > 16384;
     c.width = wide ? KV4_WIDE : KV4_W;
     const int64_t items = std::max<int64_t>(attn_tiles(rows, n_seqs, group, c.width) * kv_heads, 1);
-    int64_t pages = (max_len + KV4_PAGE - 1) / KV4_PAGE;
+    int64_t pages = (std::min<int64_t>(max_len, INT32_MAX) + KV4_PAGE - 1) / KV4_PAGE;    // lengths have 32 bits
     if (window) pages = std::min<int64_t>(pages, ((int64_t)window + c.width - 2) / KV4_PAGE + 2);
     int64_t per = 128;
     if (!wide) per = items >= 512 ? 64 : pages <= 16 ? 16 : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);

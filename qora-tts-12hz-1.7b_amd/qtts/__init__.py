@@ -189,8 +189,6 @@ class Context:
             raise QttsError(rc, "qtts_ctx_create failed (no HIP device?)")
         self.h = h
         self.device = device
-        self._kv4_need = c_int64()
-        self._kv4_need_at = ctypes.addressof(self._kv4_need)
         self._keep = []
         self.dec_codebooks = 16
 

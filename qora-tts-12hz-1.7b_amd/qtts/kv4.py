@@ -256,9 +256,8 @@ def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, m
             _table(table, n, device), PAGE * columns if max_len is None else max_len, 1 / math.sqrt(dim) if scale is None else scale,
             window)
     a = _ATTENTION.pack(*head, 0, 0)
-    need = self._kv4_need
-    need.value = 0
-    self.lib.qtts_kv4_attention_workspace(a, self._kv4_need_at)      # what it refuses the call itself names
+    need = ctypes.c_int64()
+    self.lib.qtts_kv4_attention_workspace(a, ctypes.addressof(need))      # what it refuses the call itself names
     if need.value:
         workspace = q.new_empty(need.value, dtype=_torch.uint8)
         a = _ATTENTION.pack(*head, workspace.data_ptr(), need.value)

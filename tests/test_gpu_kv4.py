@@ -4,6 +4,8 @@ block tables, norms and rotation with the store, read-back, attention.
 Codes and scales are compared exactly.  Error bounds of rows are derived where
 they are used; a type's half step is EPS relative to the value.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -296,6 +298,25 @@ def test_values_at_the_borders(ctx, kind):
     for g, w in zip(got, want):
         assert np.array_equal(host(g), w, equal_nan=True)
     assert np.isnan(host(got[0])[7, 1]).all() and not np.isnan(host(got[0])[7, 0]).any() and (host(got[1])[8, 0] == 0).all()
+
+
+def test_values_next_to_a_half(ctx):
+    """Halves between codes, exactly and by one f32 step either way, for scales
+    of 8 bits and either sign."""
+    r = np.random.default_rng(5)
+    d = (r.integers(128, 256, (64, 2, 2, 4, 1)) * 2.0 ** r.integers(-12, 4, (64, 2, 2, 4, 1)) * r.choice([-1, 1], (64, 2, 2, 4, 1)))
+    x = (d * (r.integers(-15, 16, (64, 2, 2, 4, 32)) / 2)).astype(np.float32)
+    x = np.nextafter(x, x + r.integers(-1, 2, x.shape).astype(np.float32), dtype=np.float32)
+    x[..., :1] = -8 * d                  # the extreme: code 0
+    x = x.reshape(64, 2, 2, 128).astype(np.float64)
+    t = torch.as_tensor(x).to(torch.float32).to(DEV)
+    k, v = t[:, 0].contiguous(), t[:, 1].contiguous()
+    pool = Pool(1, 2, 128)
+    cache = qtts.Kv4Cache(dev(pool.b), 2, 128)
+    ctx.qk_norm_rope(torch.zeros_like(k), k, v=v, cache=cache, slots=dev(np.arange(64)))
+    pool.put(np.arange(64), host(k), host(v))
+    for g, w in zip(ctx.kv4_gather(cache, dev(np.arange(64)), torch.float32), pool.get(np.arange(64))):
+        assert np.array_equal(host(g), w)
 
 
 # ---------------------------------------------------------------------------
@@ -810,6 +831,32 @@ def test_two_graphs_of_split_calls(ctx):
         torch.cuda.synchronize()
         for _, out, want, _, _ in runs:
             assert torch.equal(out, want)
+
+
+def test_calls_from_two_threads(ctx):
+    """Calls that need workspaces of different sizes, made at the same time."""
+    jobs = []
+    for i, n in enumerate((4000, 1500, 70)):
+        sv = Served([n], 1, 128, seed=50 + i)
+        q = torch.randn((1, 8, 128), generator=torch.Generator().manual_seed(i)).to(DEV)
+        args = (q, sv.cache, i32(sv.table), i32([0, 1]), i32([n]))
+        jobs.append((args, ctx.kv4_attention(*args)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(args, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(200):
+                out = ctx.kv4_attention(*args)
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(out, want):
+                wrong.append(args[-1])
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_calls_repeat_bit_for_bit(ctx):

@@ -169,6 +169,7 @@ def test_workspace_grows_with_the_split_only():
     assert need(rows=1, n_seqs=1, max_len=1024) == 0          # four pages for each wave
     assert need(rows=4096, n_seqs=4096, max_len=4096) == 0    # the sequences fill the card
     assert need(rows=1, n_seqs=1, max_len=1 << 40) < 1 << 25
+    assert need(rows=1, n_seqs=1, max_len=2 ** 63 - 1) == need(rows=1, n_seqs=1, max_len=2 ** 31 - 1)
 
 
 def test_reference_codes():
