@@ -446,6 +446,10 @@ int qtts_prefill_custom_voice(qtts_ctx *ctx, const uint32_t *text_tokens, int64_
  * caller's: two calls that may run at the same time, graph replays among them,
  * need two.
  *
+ * A call takes at most 2^27 rows x heads (qtts_kv4_gather 2^26 slots x kv
+ * heads), attention also at most 2^22 sequences x kv heads
+ * (QTTS_ERR_CAPACITY).
+ *
  * With QTTS_CHECK_ONLY the arguments are checked and nothing is enqueued; ctx
  * may then be NULL and no device is needed. */
 #define QTTS_CHECK_ONLY 8

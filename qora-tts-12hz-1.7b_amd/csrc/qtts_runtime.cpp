@@ -2006,7 +2006,8 @@ extern "C" int qtts_qk_norm_rope(qtts_ctx *c, const qtts_qk_norm_rope_args *a, v
     if (D != 64 && D != 128) return fail(c, QTTS_ERR_UNSUPPORTED, "heads of 64 or 128, not %d", D);
     if (a->rows < 0 || a->n_heads < 1 || a->n_kv_heads < 1 || a->n_heads % a->n_kv_heads)
         return fail(c, QTTS_ERR_INVALID, "%lld rows, %d / %d heads", (long long)a->rows, a->n_heads, a->n_kv_heads);
-    if (a->rows > (1 << 30) / (int64_t)a->n_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^30 rows x heads a call");
+    // a launch has fewer than 2^32 threads
+    if (a->rows > (1 << 27) / (int64_t)a->n_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 rows x heads a call");
     RCHK(check_rows(c, "q", a->q, a->rows, a->n_heads, D, a->q_stride, dt));
     RCHK(check_rows(c, "k", a->k, a->rows, a->n_kv_heads, D, a->k_stride, dt));
     RCHK(check_rows(c, "q_out", a->q_out, a->rows, a->n_heads, D, a->q_out_stride, dt));
@@ -2059,7 +2060,7 @@ extern "C" int qtts_kv4_gather(qtts_ctx *c, const qtts_kv4 *cache, const int64_t
     RCHK(check_dtype(c, dtype));
     RCHK(check_kv4(c, cache));
     if (n < 0 || (n && !slots) || !kv4_aligned(slots, 8)) return fail(c, QTTS_ERR_INVALID, "slots null or not aligned, or a negative count");
-    if (n > (1 << 27) / (int64_t)cache->n_kv_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^27 slots x heads a call");
+    if (n > (1 << 26) / (int64_t)cache->n_kv_heads) return fail(c, QTTS_ERR_CAPACITY, "at most 2^26 slots x heads a call");
     const int64_t bytes = n * cache->n_kv_heads * cache->head_dim * kv4_size(dtype);
     if (!kv4_aligned(K, (size_t)(4 * kv4_size(dtype))) || !kv4_aligned(V, (size_t)(4 * kv4_size(dtype))))
         return fail(c, QTTS_ERR_INVALID, "K and V must be aligned to four elements");

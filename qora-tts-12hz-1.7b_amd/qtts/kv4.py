@@ -4,7 +4,8 @@ qtts_kv4_gather, qtts_kv4_attention of include/qtts.h).
 
 Each call only enqueues kernels, on torch's current stream of the context's
 device, and may be captured into a graph.  Results and workspaces come from
-torch's allocator unless `out` arguments are given.
+torch's allocator unless `out` arguments are given.  They are operators for
+serving: no gradient passes through them.
 
 A decode step makes these calls in every layer, so a call's way to its launch
 counts as its kernel does: arguments are packed into the C structs' bytes

@@ -457,6 +457,21 @@ def test_attention_scales(ctx, kind, scale, qscale):
     attend(ctx, Served([150], 1, 64, seed=9), [2], 2, kind, scale=scale, qscale=qscale)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,H", [(5, 6), (150, 120), (420, 120)])
+def test_attention_query_without_a_value(ctx, kind, rows, H):
+    """NaN and infinite query values: NaN for their row and head, and only there."""
+    sv = Served([430], 1, 64, seed=60)
+    q = torch.randn((rows, H, 64), generator=torch.Generator().manual_seed(9)).to(TYPES[kind]).to(DEV)
+    args = (sv.cache, i32(sv.table), i32([0, rows]), i32([430]))
+    want, mag, big = kv4_ref.attention(host(q), sv.pool, sv.table, [0, rows], [430], 0.125, 0)
+    q[1, 2, 5], q[rows - 1, 0, 63], q[3, 5, 0] = float("nan"), float("inf"), -float("inf")
+    got, bad = host(ctx.kv4_attention(q, *args)), np.zeros((rows, H), bool)
+    bad[[1, rows - 1, 3], [2, 0, 5]] = True
+    assert np.isnan(got[bad]).all()
+    compare(got[~bad], want[~bad], mag[~bad], big[~bad], kind, [430])
+
+
 def test_attention_more_rows_than_positions(ctx):
     """Rows whose position lies before the sequence see nothing: zero."""
     sv = Served([3, 0], 2, 64, seed=10)

@@ -153,6 +153,16 @@ def test_attention_refuses_bad_caches(c, code):
     assert LIB.qtts_kv4_attention_workspace(ctypes.byref(attention_args(cache(**c))), ctypes.byref(n)) == code
 
 
+@pytest.mark.parametrize("rows,over", [((1 << 27) // 16, False), ((1 << 27) // 16 + 1, True)])
+def test_rows_that_a_launch_can_have(rows, over):
+    """16 heads: 2^27 rows x heads; what is below is refused for its overlaps
+    only, the addresses here being close together."""
+    assert (post(rows=rows) == qtts.ERR_CAPACITY) == over
+    assert (attend(cache(), rows=rows) == qtts.ERR_CAPACITY) == over
+    n = (1 << 26) // 8 + over
+    assert (LIB.qtts_kv4_gather(None, ctypes.byref(cache()), at(3), n, 0, at(1), at(2), None, qtts.CHECK_ONLY) == qtts.ERR_CAPACITY) == over
+
+
 def test_without_context_only_checks():
     assert LIB.qtts_kv4_attention(None, ctypes.byref(attention_args(cache())), None, 0) == qtts.ERR_INVALID
     assert LIB.qtts_kv4_gather(None, ctypes.byref(cache()), at(3), 5, 0, at(1), at(2), None, 0) == qtts.ERR_INVALID
