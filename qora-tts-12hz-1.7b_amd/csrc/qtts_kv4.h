@@ -83,7 +83,7 @@ struct Kv4Cut {
     int width, chunk, splits;
     int64_t parts;                   // partial results that the workspace holds; 0: nothing is split
 };
-Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window);
+Kv4Cut kv4_attn_cut(bool f32, int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window);
 hipError_t enqueue_kv4_attn(const Kv4Attn &a, int dtype, int D, int width, hipStream_t s);
 
 }  // namespace qtts

@@ -999,17 +999,24 @@ __device__ __forceinline__ void page_values(Running<D> (&s)[1], const Unpack &un
 }
 
 // Attention of 16 columns of one kv head over a share of the tile's pages, the
-// four waves taking them in turn and joining through LDS.  64 sequences of 1365 to
+// waves taking them in turn and joining through LDS.  64 sequences of 1365 to
 // 4096 positions, 8 kv heads of 128: 200 MB in 45 us, 4.4 TB/s, nine tenths of a
 // copy; a page costs a wave about 520 vector instructions (four fifths of them
-// unpack codes) and 32 products, nearly as long for a SIMD as its bytes take to come.  One sequence of 300 positions 11 us: tile, query, table entry and
+// unpack codes) and 32 products, nearly as long for a SIMD as its bytes take to come.  One sequence of 300 positions 8.6 us: tile, query, table entry and
 // page are waited for one after the other.
-template <class T, int D>
-__global__ void __launch_bounds__(256, 3)
+//
+// Eight waves where there are no more workgroups than CUs: half the pages one
+// after the other.  28 sequences of 3000 positions 22 us, with four waves in three
+// parts 29; where there are more, two workgroups of four waves share a CU
+// better (64 of 1365 to 4096 positions 36 us, eight waves 46).  f32 queries of 128
+// need 185 registers: two waves a SIMD without spills, not three with 28 (64
+// sequences of 4096, f32, 40 us and 60).
+template <class T, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || (std::is_same<T, float>::value && D == 128) ? 2 : 3)
 k_kv4_attn(Kv4Attn a)
 {
     constexpr int W = KV4_W, LD = D + 4;
-    __shared__ float so[4][W][LD], sm[4][W], sl[4][W];
+    __shared__ float so[WAVES][W][LD], sm[WAVES][W], sl[WAVES][W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kg = lane >> 4;
     const int ti = blockIdx.x / a.cache.heads, hk = blockIdx.x % a.cache.heads, sp = blockIdx.y;
@@ -1029,13 +1036,13 @@ k_kv4_attn(Kv4Attn a)
     const int32_t *table = a.table + (int64_t)t.b * a.table_stride;
     const Unpack un;
     const LaneAt<D> at(r, kg);
-    const int n = (pe - pb - wave + 3) / 4;      // this wave's pages: pb + wave + 4 i
+    const int n = (pe - pb - wave + WAVES - 1) / WAVES;      // this wave's pages: pb + wave + WAVES i
     int ids = 0;                                 // of 64 of them, one a lane
     const uint8_t *blk = nullptr;
     int held = 0;                                // positions whose values count
     const auto find = [&](int i) {
-        const int page = pb + wave + 4 * i;
-        if ((i & 63) == 0) ids = page + 4 * lane < pe ? table[page + 4 * lane] : -1;
+        const int page = pb + wave + WAVES * i;
+        if ((i & 63) == 0) ids = page + WAVES * lane < pe ? table[page + WAVES * lane] : -1;
         int id = __builtin_amdgcn_readlane(ids, i & 63);
         held = t.len;
         if (id < 0 || id >= a.cache.n_pages) {   // what sees this page is NaN, and for the others its values are zero
@@ -1053,7 +1060,7 @@ k_kv4_attn(Kv4Attn a)
     for (int i = 0; i < n; i++) {
         PageV<D> gv;
         load_page(gv, blk, at);
-        const int key0 = (pb + wave + 4 * i) * KV4_PAGE, count = held;
+        const int key0 = (pb + wave + WAVES * i) * KV4_PAGE, count = held;
         f32x4 x[1][4];
         __builtin_amdgcn_sched_barrier(0);
         page_scores<T, D>(x[0], un, gk, q);
@@ -1071,7 +1078,13 @@ k_kv4_attn(Kv4Attn a)
     if (poisoned) s.l = __builtin_nanf("");
     if (kg == 0) sm[wave][r] = s.m, sl[wave][r] = s.l;
     __syncthreads();
-    float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    const auto largest = [&](int c) {
+        float m = sm[0][c];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) m = fmaxf(m, sm[w][c]);
+        return m;
+    };
+    const float M = largest(r);
     const float f = s.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.m - M);
 #pragma unroll
     for (int e = 0; e < 4; e++)
@@ -1081,14 +1094,14 @@ k_kv4_attn(Kv4Attn a)
                 f32x4{s.o[i][e], s.o[i + 1][e], s.o[i + 2][e], s.o[i + 3][e]} * f;
     __syncthreads();
     const int64_t pi = ((int64_t)ti * a.cache.heads + hk) * a.splits + sp;
-    for (int e = threadIdx.x; e < W * D / 4; e += 256) {
+    for (int e = threadIdx.x; e < W * D / 4; e += 64 * WAVES) {
         const int c = e / (D / 4), d = e % (D / 4) * 4, col = t.cb + c;
         if (col >= t.ncols) break;
         f32x4 o = {0, 0, 0, 0};
         float l = 0.0f;
-        const float Mc = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+        const float Mc = largest(c);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < WAVES; w++) {
             o += *(const f32x4 *)&so[w][c][d];
             l += sm[w][c] == -INFINITY ? 0.0f * sl[w][c] : sl[w][c] * __builtin_amdgcn_exp2f(sm[w][c] - Mc);
         }
@@ -1369,33 +1382,40 @@ static int64_t attn_tiles(int64_t rows, int n_seqs, int group, int W) { return k
 // workgroups of a tile.
 //
 // The wide tiles unpack a page once for 128 columns, but cost the same for a
-// few and take a page longer (1.9 us, 16 columns 0.9): they pay where three
-// tiles of 16 columns do not hold a sequence's and there are enough to fill the
-// card.  16 columns / wide, in us, bf16, 8 kv heads of two: 64 sequences of 400
-// positions with 16, 24, 28, 64 rows each 23 / 29, 29 / 29, 36 / 30, 63 / 39; of
-// 2048 positions, 8 sequences of 64, 128, 256 rows 28 / 52, 48 / 50, 90 / 54, 32
-// sequences of 28, 32, 40, 128 rows 50 / 51, 52 / 52, 62 / 53, 174 / 93; one of
-// 4000 positions with 2000 rows 136 / 86.  f32 rows change over at the same sizes.
+// few and take a page longer (1.9 us, 16 columns 0.9): they pay where three tiles
+// of 16 columns (f32: four) do not hold a sequence's and there are enough to fill
+// the card.  16 columns / wide, in us, 8 kv heads of two:
+//   64 sequences of 400, 24, 28, 64 rows each  30 / 29, 35 / 29, 62 / 37
+//     of 1000, f32, 32, 40, 64 rows            66 / 72, 80 / 74, 124 / 82
+//   32 of 2048, 28, 40, 128 rows               49 / 49, 59 / 51, 168 / 93
+//     f32, 32, 40, 128 rows                    60 / 72, 73 / 72, 216 / 140
+//   8 of 2048, 64, 128, 256 rows               28 / 49, 48 / 51, 85 / 53
+//     f32, 128, 256 rows                       59 / 73, 109 / 77
 //
 // Splitting a tile's pages costs a second kernel (5 us, and its launch), and
-// pays where workgroups are few: 16 sequences of 16000 positions in 1024 parts 45
-// us, in 256 81; 64 of 1365 to 4096, 512 workgroups, 45 whole and 61 in two.  So
-// up to 16 pages, four for each of a workgroup's waves, stay whole (one sequence
-// of 700 11 us, in two 15), and so do shorter ones than 64 pages where the card
-// is full without, and all up to 128 on wide tiles (16 sequences of 64 rows on
-// 2048 positions 51 us, in two 72); longer ones are split for the sake of the
-// shorter ones beside them.
-Kv4Cut kv4_attn_cut(int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
+// pays where workgroups are few and the way is long: 16 sequences of 16000
+// positions in 1024 parts 45 us, in 256 81.  Whole stay
+// - up to 24 pages, and the more the more workgroups of eight waves there are:
+//   whole / split, one sequence of 1500 13 / 15, of 2000 15 / 15, 16 of 2500 19 / 20, of
+//   3000 21 / 20, 28 of 3000 22 / 29, of 4000 27 / 34;
+// - up to 16 pages of more workgroups than CUs, of four waves, and up to 64 where
+//   those fill the card twice (64 of 1365 to 4096 45, in two 61);
+// - up to 128 on wide tiles (16 of 2048, 64 rows each, 51, in two 72).
+// Longer ones are split there too, for the sake of the shorter ones beside them.
+Kv4Cut kv4_attn_cut(bool f32, int64_t rows, int n_seqs, int group, int kv_heads, int64_t max_len, int window)
 {
     Kv4Cut c{};
     const int64_t cols = n_seqs ? rows * group / n_seqs : 0;     // of an average sequence
-    const bool wide = cols > 48 && rows * group * kv_heads > 16384;
+    const bool wide = f32 ? cols > 64 && rows * group * kv_heads > 20480 : cols > 48 && rows * group * kv_heads > 16384;
     c.width = wide ? KV4_WIDE : KV4_W;
     const int64_t items = std::max<int64_t>(attn_tiles(rows, n_seqs, group, c.width) * kv_heads, 1);
     int64_t pages = (std::min<int64_t>(max_len, INT32_MAX) + KV4_PAGE - 1) / KV4_PAGE;    // lengths have 32 bits
     if (window) pages = std::min<int64_t>(pages, ((int64_t)window + c.width - 2) / KV4_PAGE + 2);
     int64_t per = 128;
-    if (!wide) per = items >= 512 ? 64 : pages <= 16 ? 16 : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);
+    if (!wide) {
+        const int64_t whole = items <= ROUND ? 24 + (items - 8) / 6 : 16;
+        per = items >= 512 ? 64 : pages <= whole ? whole : std::max<int64_t>((items * pages / 1024 + 3) / 4 * 4, 8);
+    }
     per = std::max<int64_t>(per, (pages + 63) / 64);
     c.chunk = (int)std::min<int64_t>(per, INT32_MAX / KV4_PAGE);
     c.splits = (int)std::max<int64_t>(1, (pages + per - 1) / per);
@@ -1419,8 +1439,10 @@ static hipError_t launch_attn(const Kv4Attn &a, int width, hipStream_t s)
         hipLaunchKernelGGL((k_kv4_attn_rows<T, D, 2>), grid, dim3(512), 0, s, a);
     else if (wide)
         hipLaunchKernelGGL((k_kv4_attn_rows<T, D, 1>), grid, dim3(256), 0, s, a);
+    else if ((int64_t)grid.x * grid.y <= ROUND)
+        hipLaunchKernelGGL((k_kv4_attn<T, D, 8>), grid, dim3(512), 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv4_attn<T, D>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv4_attn<T, D, 4>), grid, dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     // a workgroup a column of an average sequence's tile

@@ -2104,7 +2104,8 @@ static int check_kv4_attention(qtts_ctx *c, const qtts_kv4_attention_args *a)
 
 static Kv4Cut attention_cut(const qtts_kv4_attention_args *a)
 {
-    return kv4_attn_cut(a->rows, a->n_seqs, a->n_heads / a->cache->n_kv_heads, a->cache->n_kv_heads, a->max_len, a->window);
+    return kv4_attn_cut(a->dtype == QTTS_F32, a->rows, a->n_seqs, a->n_heads / a->cache->n_kv_heads, a->cache->n_kv_heads,
+                        a->max_len, a->window);
 }
 // Bytes of a call's partial results: maxima and sums, then rows.
 static int64_t parts_bytes(const Kv4Cut &c, int head_dim) { return c.parts * c.width * (2 + head_dim) * 4; }

@@ -458,7 +458,7 @@ def test_attention_scales(ctx, kind, scale, qscale):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("rows,H", [(5, 6), (150, 120), (420, 120)])
+@pytest.mark.parametrize("rows,H", [(5, 6), (180, 120), (420, 120)])
 def test_attention_query_without_a_value(ctx, kind, rows, H):
     """NaN and infinite query values: NaN for their row and head, and only there."""
     sv = Served([430], 1, 64, seed=60)
@@ -542,10 +542,11 @@ def test_attention_no_rows_and_no_sequences(ctx):
     assert bool((out == 2).all())
 
 
-# More than 48 columns a sequence and 16384 in all take tiles of 128 columns.
+# More than 48 columns a sequence and 16384 in all (f32: 64 and 20480) take
+# tiles of 128 columns.
 
 # sequences, rows of each, query heads, kv heads, head width
-WIDE = [([150, 257, 131], [150, 131, 128], 41, 1, 128),           # 137 tiles: two groups of waves a tile
+WIDE = [([150, 257, 131], [150, 131, 128], 51, 1, 128),           # 165 tiles: two groups of waves a tile
         ([300, 0, 64, 200], [190, 0, 1, 180], 60, 2, 64),
         ([400, 450], [400, 400], 66, 2, 128),                    # 414 tiles: one
         ([65, 500, 129], [65, 480, 1], 98, 1, 64)]
@@ -566,17 +567,17 @@ def test_attention_wide_tiles_split(ctx, kind):
     """Pages past a workgroup's 128 go to others; the short sequence beside is
     not split."""
     say("wide split", kind)
-    attend(ctx, Served([8700, 50], 1, 64, seed=30), [70, 50], 140, kind)
+    attend(ctx, Served([8700, 50], 1, 64, seed=30), [70, 50], 180, kind)
 
 
-@pytest.mark.parametrize("rows", [140, 420])
+@pytest.mark.parametrize("rows", [180, 420])
 def test_attention_wide_tiles_sharp_and_flat(ctx, rows):
     for scale in (-0.5, 1e-4, 3.0):
         say("wide", rows, scale)
         attend(ctx, Served([420], 1, 64, seed=31), [rows], 120, "f32", scale=scale)
 
 
-@pytest.mark.parametrize("rows", [140, 420])
+@pytest.mark.parametrize("rows", [180, 420])
 @pytest.mark.parametrize("entry", [-1, 2 ** 31 - 1])
 def test_attention_wide_tiles_bad_pages(ctx, rows, entry):
     """NaN for the rows that see the page, and for no other."""
@@ -594,7 +595,7 @@ def test_attention_wide_tiles_bad_pages(ctx, rows, entry):
         compare(got[~sees], want[~sees], mag[~sees], big[~sees], "f32", [420])
 
 
-@pytest.mark.parametrize("rows,HK", [(150, 1), (450, 1)])
+@pytest.mark.parametrize("rows,HK", [(180, 1), (450, 1)])
 def test_attention_wide_tiles_nan_and_empty_rows(ctx, rows, HK):
     """Rows before the sequence are zero; a NaN in a position reaches the rows
     that see it."""
@@ -616,10 +617,10 @@ def test_attention_wide_tiles_nan_and_empty_rows(ctx, rows, HK):
 
 def test_attention_wide_tiles_short_table_and_bad_sums(ctx):
     sv = Served([128], 1, 64, seed=34, columns=2)
-    q = torch.randn((150, 120, 64), generator=torch.Generator().manual_seed(4)).to(DEV)
-    got = ctx.kv4_attention(q, sv.cache, i32(sv.table), i32([0, 150]), i32([130]))
-    assert not torch.isnan(got[:148]).any() and torch.isnan(got[148:]).all()
-    for row_start, length in (([0, 151], 64), ([150, 0], 64), ([-5, 150], 64), ([0, 150], -1), ([0, 150], 2 ** 31 - 1)):
+    q = torch.randn((180, 120, 64), generator=torch.Generator().manual_seed(4)).to(DEV)
+    got = ctx.kv4_attention(q, sv.cache, i32(sv.table), i32([0, 180]), i32([130]))
+    assert not torch.isnan(got[:178]).any() and torch.isnan(got[178:]).all()
+    for row_start, length in (([0, 181], 64), ([180, 0], 64), ([-5, 180], 64), ([0, 180], -1), ([0, 180], 2 ** 31 - 1)):
         out = torch.full_like(q, 9.0)
         ctx.kv4_attention(q, sv.cache, i32(sv.table), i32(row_start), i32([length]), out=out)
         assert bool((out == 9).all())
@@ -640,6 +641,25 @@ def test_many_sequences_find_their_tiles(ctx):
     held = pool.get(np.arange(70) * PAGE)[1][:, 0, 0]
     want = held[table[np.repeat(np.arange(n), fresh), 0]][:, None, None]      # constant values: the average is the value
     assert (np.abs(got - want) <= want * 2.0 ** -21).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("H,HK,window", [(16, 8, 0), (21, 7, 40)])
+def test_attention_more_workgroups_than_cus(ctx, kind, H, HK, window):
+    """Heads of 128 on four waves a tile."""
+    say("many", kind, H, HK, window)
+    r = np.random.default_rng(H)
+    lengths = r.integers(0, 300, 45).tolist()
+    attend(ctx, Served(lengths, HK, 128, seed=H), r.integers(1, 4, 45).tolist(), H, kind, window=window)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_attention_many_sequences_split(ctx, kind):
+    """Two long sequences among short ones: theirs alone are split."""
+    say("many split", kind)
+    lengths = np.random.default_rng(3).integers(1, 60, 34)
+    lengths[[4, 30]] = 1500, 1437
+    attend(ctx, Served(lengths.tolist(), 8, 64, seed=3), [1] * 34, 16, kind, max_len=1500)
 
 
 # More than 256 workgroups: tiles are taken in order of their pages, if there
