@@ -20,6 +20,7 @@ import sys
 from .hostdesc import Kv4
 
 PAGE = 64
+WHOLE = 16 * PAGE            # attention over no more positions is never split: it needs no workspace
 _TABLES = struct.Struct("@iiPPPqPqPPPPqP")                 # qtts_kv4_tables_args
 _POST = struct.Struct("@iiiiqPPPqqqPPqqPPfiPPqPPP")        # qtts_qk_norm_rope_args
 _ATTENTION = struct.Struct("@iiqPPqqPiiPPPqqfiPq")         # qtts_kv4_attention_args
@@ -252,16 +253,18 @@ def attention(self, q, cache, table, row_start, lengths, scale=None, window=0, m
     else:
         out_stride = _rows("out", out, shape, dtype, device)
     columns = table.shape[1] if table.dim() == 2 else 0
+    if max_len is None:
+        max_len = PAGE * columns
     head = (code, heads, rows, q.data_ptr(), out.data_ptr(), q_stride, out_stride, cache.address, n, columns,
             _vector("row_start", row_start, n + 1, i32, device), _vector("lengths", lengths, n, i32, device), table.data_ptr(),
-            _table(table, n, device), PAGE * columns if max_len is None else max_len, 1 / math.sqrt(dim) if scale is None else scale,
-            window)
+            _table(table, n, device), max_len, 1 / math.sqrt(dim) if scale is None else scale, window)
     a = _ATTENTION.pack(*head, 0, 0)
-    need = ctypes.c_int64()
-    self.lib.qtts_kv4_attention_workspace(a, ctypes.addressof(need))      # what it refuses the call itself names
-    if need.value:
-        workspace = q.new_empty(need.value, dtype=_torch.uint8)
-        a = _ATTENTION.pack(*head, workspace.data_ptr(), need.value)
+    if max_len > WHOLE:
+        need = ctypes.c_int64()
+        self.lib.qtts_kv4_attention_workspace(a, ctypes.addressof(need))      # what it refuses the call itself names
+        if need.value:
+            workspace = q.new_empty(need.value, dtype=_torch.uint8)
+            a = _ATTENTION.pack(*head, workspace.data_ptr(), need.value)
     rc = self.lib.qtts_kv4_attention(self.h, a, _stream(device), 0)
     if rc:
         self._check(rc)

@@ -182,6 +182,17 @@ def test_workspace_grows_with_the_split_only():
     assert need(rows=1, n_seqs=1, max_len=2 ** 63 - 1) == need(rows=1, n_seqs=1, max_len=2 ** 31 - 1)
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("window", [0, 70, 5000])
+def test_short_calls_need_no_workspace(dtype, window):
+    """What the binding takes for granted up to qtts.kv4.WHOLE positions."""
+    n = ctypes.c_int64(-1)
+    for rows in (0, 1, 7, 300, 5000, 100000):
+        for seqs in (0, 1, 2, 9, 33, 64, 257, 4000):
+            a = attention_args(cache(), dtype=dtype, rows=rows, n_seqs=seqs, max_len=qtts.kv4.WHOLE, window=window)
+            assert LIB.qtts_kv4_attention_workspace(ctypes.byref(a), ctypes.byref(n)) == qtts.OK and n.value == 0
+
+
 def test_reference_codes():
     """Known answers of the format: the extreme value is code 0, steps of an
     eighth, halves to even, saturation, and what 8 significant bits keep."""
