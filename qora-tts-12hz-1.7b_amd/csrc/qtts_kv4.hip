@@ -1116,12 +1116,15 @@ k_kv4_attn(Kv4Attn a)
     }
 }
 
-// A page of a prompt's tile as a thread loads it: each of four waves takes one
-// K tile (rows 4r + share) and one V block (positions 16 kg + 4 share .. + 3),
-// so that each code of the page is unpacked once for all four.
+// A page of a prompt's tile as a thread loads it, each code of it unpacked once
+// for four waves.  Each takes one K tile (rows 4r + share) and of V, with D = 128,
+// eight positions (16 kg + 8 (share / 2) ..) of half the columns, which are whole
+// 16 bytes of four fragments (as halves of eight, their writes met in LDS banks: one
+// prompt of 4000 positions 108 us, now 106); with D = 64 four positions of all
+// columns, halves of four fragments.
 template <int D>
 struct PageShare {
-    uint32_t k[D / 32], v[D / 32], vs[2];
+    uint32_t k[D / 32], v[D / 32], vs[D / 32];
     uint16_t ks;
     int held;                        // positions whose values count
 };
@@ -1198,10 +1201,17 @@ k_kv4_attn_rows(Kv4Attn a)
         }
         const uint8_t *blk = a.cache.base + id * a.cache.stride + (int64_t)hk * kv4_block(D);
         load_words<D>(g.k, blk + share * (kv4_k_at(D, 1) - kv4_k_at(D, 0)) + at.k);
-        load_words<D>(g.v, blk + share * (kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0)) + at.v);
         g.ks = *(const uint16_t *)(blk + share * 2 + at.ks);
-        const uint2 vs = *(const uint2 *)(blk + share * 8 + at.vs);
-        g.vs[0] = vs.x, g.vs[1] = vs.y;
+        constexpr int block = kv4_v_at(D, 4, 0) - kv4_v_at(D, 0, 0);
+        if constexpr (D == 128) {
+            const uint8_t *v = blk + share / 2 * 2 * block + share % 2 * 8 + at.v;
+            load_words<64>(g.v, v);
+            load_words<64>(g.v + 2, v + block);
+            load_words<128>(g.vs, blk + share / 2 * 16 + at.vs);
+        } else {
+            load_words<D>(g.v, blk + share * block + at.v);
+            load_words<64>(g.vs, blk + share * 8 + at.vs);
+        }
     };
     const auto stage = [&](PageShare<D> &g, int it) {
         const int key0 = (pb + HALVES * it + half) * KV4_PAGE;
@@ -1213,16 +1223,18 @@ k_kv4_attn_rows(Kv4Attn a)
             unpack8(un, g.k[j], ks, k);
             to[share * (D / 32) + j][lane] = u32x4{k[0], k[1], k[2], k[3]};
         }
-        if (key0 + KV4_PAGE > g.held) mask_values(g.vs, key0 + 16 * kg + 4 * share, g.held);
+        const int first = key0 + 16 * kg + (D == 128 ? 8 * (share / 2) : 4 * share);
+        if (key0 + KV4_PAGE > g.held) mask_values(g.vs, first, g.held);
+        uint32_t v[D / 32][4];
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) {
-            uint32_t v0[4], v1[4];
-            unpack8(un, g.v[2 * c], as_h2(g.vs[0]), v0);
-            unpack8(un, g.v[2 * c + 1], as_h2(g.vs[1]), v1);
+        for (int h = 0; h < D / 32; h++) unpack8(un, g.v[h], as_h2(g.vs[h]), v[h]);
+        u32x4 (*const tv)[64] = to + KF + share / 2 * (D / 16);
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-                *((uint2 *)&to[KF + share / 2 * (D / 16) + 4 * c + n][lane] + share % 2) = make_uint2(v0[n], v1[n]);
-        }
+        for (int n = 0; n < 4; n++)
+            if constexpr (D == 128)
+                tv[4 * (share % 2) + n][lane] = u32x4{v[0][n], v[1][n], v[2][n], v[3][n]};
+            else
+                *((uint2 *)&tv[n][lane] + share % 2) = make_uint2(v[0][n], v[1][n]);
     };
 
     // a page too many for the second half is fetched as none and masked for every column
