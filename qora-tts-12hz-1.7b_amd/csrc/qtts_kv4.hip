@@ -1139,8 +1139,8 @@ constexpr int DS_STAYS = 0x47F;      // sched_barrier: all but LDS instructions 
 // overlap here (48 of 4.4 cycles and four of 16.6 take their sum, from one wave or
 // from two), so a page costs what its 425 vector instructions and 64 products a
 // wave add up to, 3000 cycles, and a fifth more for waits.  Four prompts of 500
-// to 1000 rows, 29.6 GFLOP: 61 us, 485 TFLOP/s; the longest tile's 32 pages, one
-// after the other, are 52 of them.
+// to 1000 rows, 29.6 GFLOP: 59 us, 500 TFLOP/s; the longest tile's 32 pages, one
+// after the other, are 50 of them.
 //
 // HALVES 2, for no more tiles than CUs: eight waves, the second four taking every
 // other page, joined at the end.  The longest tile's way is half as long, and
